@@ -176,6 +176,126 @@ int8conv_status int8conv_launch_requant(int strategy, const int8conv_shape *shap
                                         int8_t *output, void *workspace,
                                         size_t workspace_bytes, void *stream);
 
+/* ---- products, row quantisation and group norm ----------------------------------
+ *
+ * The operators a quantised model runs between its convolutions.  Same manner
+ * as the launches above: the caller owns every buffer, launches are
+ * asynchronous on `stream` and never allocate, statuses instead of aborts.
+ * No reference counterpart. */
+
+/* Element types of operands and outputs. */
+typedef enum int8conv_dtype {
+  INT8CONV_BF16 = 0,
+  INT8CONV_FP16 = 1,
+  INT8CONV_FP32 = 2,
+  INT8CONV_INT8 = 3,
+  INT8CONV_INT32 = 4
+} int8conv_dtype;
+
+typedef enum int8conv_activation {
+  INT8CONV_ACT_NONE = 0,
+  INT8CONV_ACT_RELU = 1,      /* max(v, 0) */
+  INT8CONV_ACT_GELU = 2,      /* v * (1 + erf(v / sqrt 2)) / 2 */
+  INT8CONV_ACT_GELU_TANH = 3, /* v * (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) / 2 */
+  INT8CONV_ACT_SILU = 4       /* v / (1 + exp(-v)) */
+} int8conv_activation;
+
+#define INT8CONV_MAX_PRODUCT_K 131071 /* |int8|^2 * k stays within int32 */
+#define INT8CONV_MAX_GROUPS 1024
+#define INT8CONV_MAX_NORM_CHANNELS 8192
+
+/* One matrix product with its epilogue:
+ *   acc[i,j] = sum_k a[i,k] * b[j,k]                       exact, int32
+ *   v        = acc * row_scale[i] * col_scale[j] + bias[j] fp32
+ *   y[i,j]   = activation(v) + residual[i,j]               rounded once to y_dtype
+ * and for y_dtype INT8
+ *   y[i,j]   = clamp(round_half_even(activation(v) * (1 / out_scale)), -128, 127), NaN -> 0
+ *
+ * a is int8 [m][k] with rows lda bytes apart, b int8 [n][k] with rows ldb bytes
+ * apart (lda, ldb multiples of 16 and >= k; the bytes between k and the pitch
+ * are never used).  y has rows ldy elements apart (>= n), residual rows ldr.
+ * y and residual need the alignment of their elements only; 16-byte aligned
+ * rows are stored faster.  residual has y's type; it may be y itself (same
+ * address and pitch: y += ...), any other overlap is undefined.  Nothing
+ * outside y's m x n elements is written. */
+typedef struct int8conv_matmul {
+  int64_t m, n, k;
+  int64_t lda, ldb, ldy, ldr;
+  const float *row_scale;   /* m entries, or NULL for 1 */
+  const float *col_scale;   /* n entries (groups x n), or NULL for 1 */
+  const float *bias;        /* n entries (groups x n), or NULL for 0 */
+  const void *residual;     /* NULL for none; not with y_dtype INT8 */
+  int32_t activation;       /* int8conv_activation */
+  int32_t y_dtype;          /* BF16, FP16, FP32 or INT8 */
+  float out_scale;          /* y_dtype INT8: what one step is worth, finite and > 0 */
+} int8conv_matmul;
+
+/* m = 0 or n = 0 is OK and writes nothing.  BAD_ARGUMENT for a negative size,
+ * k outside [1, INT8CONV_MAX_PRODUCT_K], a pitch below the row or (lda, ldb)
+ * not a multiple of 16, an unknown type or activation, a residual with INT8
+ * output, or a bad out_scale; BAD_POINTER for a NULL operand or output, a or b
+ * not 16-byte aligned, or another buffer not aligned to its elements. */
+int8conv_status int8conv_launch_matmul(const int8conv_matmul *desc, const int8_t *a,
+                                       const int8_t *b, void *y, void *stream);
+
+/* The product grouped by expert: rows offsets[e] .. offsets[e+1]-1 of a (and of
+ * row_scale and y) meet b[e], expert e's int8 [n][k], which starts
+ * e * group_stride bytes into b (a multiple of 16); col_scale and bias hold n
+ * entries for each expert.  `offsets` is device memory, groups + 1 entries,
+ * ascending; experts may be empty.  Rows below offsets[0] and from
+ * offsets[groups] on are left as they were.  The kernel reads each offset as
+ * at least its predecessor and at most m, so offsets that are out of order or
+ * out of range move no access outside the buffers.  No residual
+ * (BAD_ARGUMENT).  1 <= groups <= INT8CONV_MAX_GROUPS. */
+int8conv_status int8conv_launch_grouped_matmul(const int8conv_matmul *desc, const int8_t *a,
+                                               const int8_t *b, int64_t group_stride,
+                                               const int32_t *offsets, int32_t groups, void *y,
+                                               void *stream);
+
+/* Rows of x to int8 with one scale each:
+ *   scale[i] = max_k |x[r,k]| / 127
+ *   q[i,k]   = round_half_even(x[r,k] / scale[i])       fp32, IEEE division
+ * with r = index[i], or r = i where index is NULL (then rows must be >= m).
+ * A row of zeros gives zeros and scale 0; a row that holds an infinity or a
+ * NaN gives zeros and scale NaN, so that every product of that row is NaN; an
+ * index outside [0, rows) gives zeros and scale 0.  x: BF16, FP16 or FP32
+ * [rows][k], rows ldx elements apart (>= k); q: rows ldq bytes apart (>= k),
+ * bytes from k to the pitch left as they were.  x, q, scale and index need the
+ * alignment of their elements only. */
+int8conv_status int8conv_launch_quantize_rows(int64_t m, int64_t k, int32_t x_dtype, const void *x,
+                                              int64_t rows, int64_t ldx, const int32_t *index,
+                                              int8_t *q, int64_t ldq, float *scale, void *stream);
+
+/* Group norm with an activation over n images of `pixels` positions, channels
+ * last:
+ *   v       = x[i,p,c] * scale[c]            (scale NULL: 1)
+ *   mean_g, var_g over the pixels and the channels of group g = c / (c / groups)
+ *   y       = activation((v - mean_g) / sqrt(var_g + eps) * gamma[c] + beta[c])
+ * with gamma NULL: 1, beta NULL: 0.  x is BF16, FP16, FP32 or INT32 (what a
+ * convolution launch wrote; scale is then what one step of channel c is
+ * worth), y BF16, FP16, FP32 or INT8 (with out_scale as for the products).
+ * Positions are ldx / ldy elements apart (>= channels), images pixels * ldx /
+ * pixels * ldy.  channels % groups == 0, channels <= INT8CONV_MAX_NORM_CHANNELS.
+ * y may be x itself where types and pitches are equal.  Statistics are held in
+ * fp32 as (mean, squared deviations) pairs, joined in a fixed order. */
+typedef struct int8conv_group_norm {
+  int64_t n, pixels;
+  int32_t channels, groups;
+  int64_t ldx, ldy;
+  const float *scale, *gamma, *beta; /* channels entries each, or NULL */
+  float eps;                         /* finite, >= 0 */
+  int32_t activation;
+  int32_t x_dtype, y_dtype;
+  float out_scale;
+} int8conv_group_norm;
+
+/* Device scratch of a launch, in bytes; 0 for an invalid descriptor.  Launches
+ * that may run at the same time each need their own. */
+size_t int8conv_group_norm_workspace_bytes(const int8conv_group_norm *desc);
+
+int8conv_status int8conv_launch_group_norm(const int8conv_group_norm *desc, const void *x, void *y,
+                                           void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- host buffers ------------------------------------------------------------*/
 
 /* End-to-end convolution of HOST buffers (no reference counterpart; the

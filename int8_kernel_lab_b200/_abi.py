@@ -42,6 +42,34 @@ LAYOUT_NCHW_VECT_C = 1
 LAYOUTS = {"nhwc": LAYOUT_NHWC, "nchw_vect_c": LAYOUT_NCHW_VECT_C}
 
 
+# int8conv_dtype, by torch's names
+BF16 = 0
+FP16 = 1
+FP32 = 2
+INT8 = 3
+INT32 = 4
+DTYPES = {"bfloat16": BF16, "float16": FP16, "float32": FP32, "int8": INT8, "int32": INT32}
+
+# int8conv_activation
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+class CMatmul(ctypes.Structure):
+    _fields_ = ([(f, ctypes.c_int64) for f in ("m", "n", "k", "lda", "ldb", "ldy", "ldr")]
+                + [(f, ctypes.c_void_p) for f in ("row_scale", "col_scale", "bias", "residual")]
+                + [("activation", ctypes.c_int32), ("y_dtype", ctypes.c_int32),
+                   ("out_scale", ctypes.c_float)])
+
+
+class CGroupNorm(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_int64), ("pixels", ctypes.c_int64), ("channels", ctypes.c_int32),
+                ("groups", ctypes.c_int32), ("ldx", ctypes.c_int64), ("ldy", ctypes.c_int64),
+                ("scale", ctypes.c_void_p), ("gamma", ctypes.c_void_p), ("beta", ctypes.c_void_p),
+                ("eps", ctypes.c_float), ("activation", ctypes.c_int32),
+                ("x_dtype", ctypes.c_int32), ("y_dtype", ctypes.c_int32),
+                ("out_scale", ctypes.c_float)]
+
+
 class CRequant(ctypes.Structure):
     _fields_ = [("multiplier", ctypes.c_void_p), ("exponent", ctypes.c_void_p),
                 ("zero_point", ctypes.c_int32), ("relu", ctypes.c_int32),
@@ -82,6 +110,15 @@ SIGNATURES = {
     "int8conv_launch_requant": (ctypes.c_int, [ctypes.c_int, _SP, _P, _P, _P,
                                                ctypes.POINTER(CRequant), _P, _P, ctypes.c_size_t,
                                                _P]),
+    "int8conv_launch_matmul": (ctypes.c_int, [ctypes.POINTER(CMatmul), _P, _P, _P, _P]),
+    "int8conv_launch_grouped_matmul": (ctypes.c_int, [ctypes.POINTER(CMatmul), _P, _P,
+                                                      ctypes.c_int64, _P, ctypes.c_int32, _P, _P]),
+    "int8conv_launch_quantize_rows": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
+                                                     _P, ctypes.c_int64, ctypes.c_int64, _P, _P,
+                                                     ctypes.c_int64, _P, _P]),
+    "int8conv_group_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(CGroupNorm)]),
+    "int8conv_launch_group_norm": (ctypes.c_int, [ctypes.POINTER(CGroupNorm), _P, _P, _P,
+                                                  ctypes.c_size_t, _P]),
     "int8conv_device_status": (ctypes.c_int, []),
     "int8conv_set_wait_limit_ns": (None, [ctypes.c_uint64]),
     "int8conv_debug_starve_producer": (None, [ctypes.c_int]),

@@ -151,4 +151,19 @@ int8conv_status launch_halo_impl(const int8conv_shape &s, const int8_t *x, const
 int8conv_status launch_splitk_impl(const int8conv_shape &s, const int8_t *x, const int8_t *w,
                                    const int32_t *b, int32_t *y, cudaStream_t stream);
 
+// Products, row quantisation and group norm (validated arguments, nothing
+// empty).  groups = 0: the plain product.
+int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, const int8_t *b,
+                                   int64_t group_stride, const int32_t *offsets, int32_t groups,
+                                   void *y, cudaStream_t stream);
+int8conv_status launch_quantize_rows_impl(int64_t m, int64_t k, int x_dtype, const void *x,
+                                          int64_t rows, int64_t ldx, const int32_t *index,
+                                          int8_t *q, int64_t ldq, float *scale,
+                                          cudaStream_t stream);
+// CTAs of a group norm's statistics, and the bytes of their partial results.
+int64_t group_norm_blocks(const int8conv_group_norm &d);
+size_t group_norm_workspace(const int8conv_group_norm &d);
+int8conv_status launch_group_norm_impl(const int8conv_group_norm &d, const void *x, void *y,
+                                       void *workspace, cudaStream_t stream);
+
 }  // namespace i8c

@@ -1,0 +1,792 @@
+// matmul.cu - int8 matrix products with a floating-point epilogue, plain and
+// grouped by expert:
+//   y[i,j] = act(acc * row_scale[i] * col_scale[j] + bias[j]) + residual[i,j],
+//   acc[i,j] = sum_k a[i,k] * b[j,k]   (int32, exact: k <= 131071)
+//
+// One persistent kernel, 10 warps, one CTA per SM or CTA pairs
+// (tcgen05 cta_group::2, 256-row tiles):
+//   warp 0     TMA producer: A and B tiles of 128 bytes of k, 128-byte swizzle,
+//              into an mbarrier ring.  Rows and columns past the matrices and
+//              bytes past k arrive as zeros, so no size has to divide a tile.
+//   warp 1     MMA issuer: tcgen05.mma kind::i8, int32 accumulators in TMEM,
+//              two buffers, so the epilogue of a tile runs under the next one.
+//   warps 2-9  epilogue, two warps for each TMEM lane quarter, each taking
+//              every other 32-column block: one row per thread, the column
+//              scales and biases of the tile in shared memory, the residual
+//              read straight into registers, one rounding to the output type,
+//              then a 32 x 32 block staged in swizzled shared memory and written
+//              by one TMA store (or, where the pitch or a ragged group's end
+//              does not allow one, by row segments of 16 bytes or elements).
+// A rows are loaded in boxes of 8 to 128 rows (fewer for few tokens): the tile
+// rows that no box covers keep whatever the ring held.  They are integers, so
+// they can only reach their own accumulator rows, which nothing stores.
+//
+// Grouped: A rows are sorted by expert and B is [groups][n][k].  Every CTA
+// scans the device-side offsets into a table of row tiles in shared memory, and
+// its roles walk the same list of (expert, column tile, row tile) units.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+#include <math.h>
+
+#include <mutex>
+
+#include "conv_common.h"
+#include "epilogue.cuh"
+#include "launch.h"
+#include "sm100.cuh"
+
+namespace i8c {
+
+namespace {
+
+constexpr int kBlockK = 128;                  // bytes of k per stage
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kStageBytes = 4096;             // epilogue staging per warp
+constexpr int kTableBytes = 1024;             // 128 columns x (scale, bias) per warp
+constexpr int kMaxStages = 12;
+
+struct MatmulGeom {
+  int32_t M, N;
+  int32_t kblocks;
+  int32_t bn;          // tile width (multiple of 32)
+  int32_t a_rows;      // rows of one A box (8..128)
+  int32_t n_tiles, m_tiles;
+  int32_t band;        // row tiles of one band of the tile order
+  int32_t stages;
+  int32_t tmem_cols;
+  int32_t tma_store;   // 1: whole 32 x 32 blocks leave as TMA stores
+  int32_t vec_store;   // 1: rows of y are 16-byte aligned
+  int32_t vec_res;     // 1: rows of the residual are 16-byte aligned
+  int32_t activation;
+  int32_t groups;      // 0: plain product
+  float inv_out_scale;
+  int64_t ldy, ldr;    // elements
+  const float *row_scale, *col_scale, *bias;
+  const void *residual;
+  void *y;
+  const int32_t *offsets;
+};
+
+// Shared-memory plan, identical on host and device.
+struct MatmulSmem {
+  uint32_t a_bytes, b_bytes;   // one stage, this CTA's share
+  uint32_t b_off, staging_off, table_off, bar_off, group_off, total;
+};
+
+__host__ __device__ inline MatmulSmem matmul_smem(int b_rows, int stages, int groups) {
+  MatmulSmem p;
+  p.a_bytes = kBlockM * kBlockK;
+  p.b_bytes = b_rows * kBlockK;
+  p.b_off = stages * p.a_bytes;
+  p.staging_off = p.b_off + stages * p.b_bytes;   // b_rows * 128 is a multiple of 1024
+  p.table_off = p.staging_off + kEpiWarps * kStageBytes;
+  p.bar_off = p.table_off + kEpiWarps * kTableBytes;
+  // full/empty[stages], tfull[2], tempty[2], drain, TMEM slot
+  p.group_off = p.bar_off + (2 * stages + 5) * 8 + 8;
+  p.total = 1024 + p.group_off + (groups > 0 ? (2 * groups + 2) * 4 : 0);
+  return p;
+}
+
+struct Tile {
+  int m0;      // first row
+  int m_end;   // rows at and past this one are not this tile's to store
+  int n0;      // first column
+  int group;
+};
+
+// Work units of a launch.  Plain: bands of `band` row tiles, and inside a band
+// column by column, so that the CTAs running at one time share few rows of A
+// and of B.  Grouped: expert by expert, column by column.
+template <bool GROUPED>
+__device__ __forceinline__ Tile tile_at(const MatmulGeom &g, int tile_rows, const int32_t *row_start,
+                                        const int32_t *tile_start, int u) {
+  Tile t;
+  if constexpr (GROUPED) {
+    int lo = 0, hi = g.groups;   // tile_start[lo] * n_tiles <= u < tile_start[hi] * n_tiles
+    const int at = u / g.n_tiles;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (tile_start[mid] <= at) lo = mid;
+      else hi = mid;
+    }
+    const int first = tile_start[lo];
+    const int count = tile_start[lo + 1] - first;
+    const int local = u - first * g.n_tiles;
+    const int n = local / count;
+    t.group = lo;
+    t.m0 = row_start[lo] + (local - n * count) * tile_rows;
+    t.m_end = row_start[lo + 1];
+    t.n0 = n * g.bn;
+  } else {
+    const int per_band = g.band * g.n_tiles;
+    const int b = u / per_band;
+    const int local = u - b * per_band;
+    const int left = g.m_tiles - b * g.band;
+    const int height = left < g.band ? left : g.band;
+    const int n = local / height;
+    t.group = 0;
+    t.m0 = (b * g.band + local - n * height) * tile_rows;
+    t.m_end = g.M;
+    t.n0 = n * g.bn;
+  }
+  return t;
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void commit_mma(uint64_t *bar) {
+  if constexpr (PAIR)
+    umma_commit_pair(bar, 0x3);
+  else
+    umma_commit(bar);
+}
+
+// scale, bias and activation of one 32-column block of a thread's row;
+// `table`: (scale, bias) of the block's columns, two columns per float4.
+template <int ACT>
+__device__ __forceinline__ void finish_block(uint32_t (&v)[32], float rs, const float4 *table) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float4 t = table[j];
+    const float a = fmaf(static_cast<float>(static_cast<int32_t>(v[2 * j])) * t.x, rs, t.y);
+    const float b = fmaf(static_cast<float>(static_cast<int32_t>(v[2 * j + 1])) * t.z, rs, t.w);
+    v[2 * j] = __float_as_uint(activate<ACT>(a));
+    v[2 * j + 1] = __float_as_uint(activate<ACT>(b));
+  }
+}
+
+template <int OUT>
+constexpr int out_bytes() {
+  return OUT == INT8CONV_FP32 ? 4 : OUT == INT8CONV_INT8 ? 1 : 2;
+}
+
+// 16-byte chunk `j` of row `row` in a staged block, under the TMA swizzle whose
+// span is the block's row (128, 64 or 32 bytes).
+template <int OUT>
+__device__ __forceinline__ int chunk_at(int row, int j) {
+  if constexpr (OUT == INT8CONV_FP32) return row * 8 + (j ^ (row & 7));
+  if constexpr (OUT == INT8CONV_INT8) return row * 2 + (j ^ ((row >> 2) & 1));
+  return row * 4 + (j ^ ((row >> 1) & 3));
+}
+
+// Adds the residual's 32 columns (row pointer `r`, `cols` of them inside the
+// matrix) to the block.
+template <int OUT>
+__device__ __forceinline__ void add_residual(uint32_t (&v)[32],
+                                             const typename Elem<OUT>::type *r, int cols,
+                                             bool vec) {
+  using T = typename Elem<OUT>::type;
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  if (vec && cols >= 32) {
+#pragma unroll
+    for (int j = 0; j < 32 / kPer; ++j) {
+      const uint4 raw = *reinterpret_cast<const uint4 *>(r + j * kPer);
+      const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+      for (int t = 0; t < kPer; ++t)
+        v[j * kPer + t] = __float_as_uint(__uint_as_float(v[j * kPer + t]) + Elem<OUT>::load(e[t]));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < cols) v[j] = __float_as_uint(__uint_as_float(v[j]) + Elem<OUT>::load(r[j]));
+  }
+}
+
+// One thread's 32 values, rounded, into its row of the staged block.
+template <int OUT>
+__device__ __forceinline__ void stage_row(const uint32_t (&v)[32], uint4 *stg, int row,
+                                          float inv_out_scale) {
+  auto f = [&](int i) { return __uint_as_float(v[i]); };
+  if constexpr (OUT == INT8CONV_FP32) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      stg[chunk_at<OUT>(row, j)] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  } else if constexpr (OUT == INT8CONV_INT8) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t w[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int i = 16 * j + 4 * t;
+        w[t] = pack_int8(f(i) * inv_out_scale, f(i + 1) * inv_out_scale, f(i + 2) * inv_out_scale,
+                         f(i + 3) * inv_out_scale);
+      }
+      stg[chunk_at<OUT>(row, j)] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t w[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int i = 8 * j + 2 * t;
+        w[t] = OUT == INT8CONV_BF16 ? pack_bf16(f(i), f(i + 1)) : pack_fp16(f(i), f(i + 1));
+      }
+      stg[chunk_at<OUT>(row, j)] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+// The staged block to global memory without TMA: rows [0, rows), columns
+// [0, cols) at `y` (the block's first element).
+template <int OUT>
+__device__ __forceinline__ void copy_out(const uint4 *stg, typename Elem<OUT>::type *y, int64_t ldy,
+                                         int rows, int cols, bool vec, int lane) {
+  using T = typename Elem<OUT>::type;
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  constexpr int kChunks = 32 / kPer;           // 16-byte chunks per row
+  constexpr int kRows = 32 / kChunks;          // rows per pass of the warp
+  if (vec) {
+    const int j = lane % kChunks;
+    for (int r = lane / kChunks; r < rows; r += kRows) {
+      const uint4 raw = stg[chunk_at<OUT>(r, j)];
+      T *dst = y + r * ldy + j * kPer;
+      if ((j + 1) * kPer <= cols) {
+        *reinterpret_cast<uint4 *>(dst) = raw;
+      } else {
+        const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+        for (int t = 0; t < kPer; ++t)
+          if (j * kPer + t < cols) dst[t] = e[t];
+      }
+    }
+  } else if (lane < cols) {
+    const T *e = reinterpret_cast<const T *>(stg);
+    for (int r = 0; r < rows; ++r)
+      y[r * ldy + lane] = e[chunk_at<OUT>(r, lane / kPer) * kPer + lane % kPer];
+  }
+}
+
+template <bool PAIR, bool GROUPED, int OUT>
+__global__ void __launch_bounds__(kThreads, 1)
+    matmul_kernel(const __grid_constant__ CUtensorMap tmap_a,
+                  const __grid_constant__ CUtensorMap tmap_b,
+                  const __grid_constant__ CUtensorMap tmap_y, const MatmulGeom g,
+                  const RunCtl ctl) {
+  extern __shared__ uint8_t smem_raw[];
+  // 1024-byte alignment for the 128-byte swizzle; the same offset in both CTAs
+  // of a pair.
+  uint8_t *smem = reinterpret_cast<uint8_t *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  constexpr int kTileRows = PAIR ? 2 * kBlockM : kBlockM;
+  const MatmulSmem plan = matmul_smem(PAIR ? g.bn / 2 : g.bn, g.stages, GROUPED ? g.groups : 0);
+  uint8_t *a_ring = smem;
+  uint8_t *b_ring = smem + plan.b_off;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + plan.bar_off);
+  uint64_t *empty = full + g.stages;
+  uint64_t *tfull = empty + g.stages;
+  uint64_t *tempty = tfull + 2;
+  uint64_t *drain = tempty + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+  int32_t *row_start = reinterpret_cast<int32_t *>(smem + plan.group_off);
+  int32_t *tile_start = row_start + g.groups + 1;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const WaitCtx wctx{ctl.wait_ns, ctl.status};
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
+  const bool leader = rank == 0;
+  const int first = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int step = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+
+  if (warp == 0) {
+    for (int i = lane; i < 2 * g.stages + 5; i += 32) {
+      // tempty: one arrival per epilogue warp (of both CTAs for a pair).
+      const bool te = i >= 2 * g.stages + 2 && i < 2 * g.stages + 4;
+      mbar_init(&full[i], te ? (PAIR ? 2 : 1) * kEpiWarps : 1);
+    }
+    fence_mbar_init();
+    if (lane == 0) {
+      tma_prefetch_desc(&tmap_a);
+      tma_prefetch_desc(&tmap_b);
+    }
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_alloc_pair(tmem_slot, g.tmem_cols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, g.tmem_cols);
+      tmem_relinquish();
+    }
+  }
+  int num_tiles = g.m_tiles * g.n_tiles;
+  if constexpr (GROUPED) {
+    // Nothing is read before the previous kernel in the stream is complete.
+    griddep_wait();
+    for (int i = threadIdx.x; i <= g.groups; i += kThreads) {
+      const int32_t o = __ldg(g.offsets + i);
+      row_start[i] = o < 0 ? 0 : (o > g.M ? g.M : o);
+    }
+    __syncthreads();
+    if (warp == 0) {
+      // Running maximum of the offsets, then running count of row tiles.
+      int32_t top = 0, tiles = 0;
+      if (lane == 0) tile_start[0] = 0;
+      for (int base = 0; base <= g.groups; base += 32) {
+        const int i = base + lane;
+        int32_t end = i <= g.groups ? row_start[i] : 0;
+        end = end > top ? end : top;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int32_t o = __shfl_up_sync(0xffffffffu, end, d);
+          if (lane >= d && o > end) end = o;
+        }
+        int32_t begin = __shfl_up_sync(0xffffffffu, end, 1);
+        if (lane == 0) begin = base == 0 ? end : top;   // entry 0 opens no group
+        int32_t count = i <= g.groups ? (end - begin + kTileRows - 1) / kTileRows : 0;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int32_t o = __shfl_up_sync(0xffffffffu, count, d);
+          if (lane >= d) count += o;
+        }
+        if (i <= g.groups) {
+          row_start[i] = end;
+          tile_start[i] = tiles + count;
+        }
+        top = __shfl_sync(0xffffffffu, end, 31);
+        tiles += __shfl_sync(0xffffffffu, count, 31);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();   // both CTAs' barriers are set up
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  if constexpr (GROUPED) num_tiles = tile_start[g.groups] * g.n_tiles;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------- TMA producer ----------------
+      if constexpr (!GROUPED) griddep_wait();
+      int stage = 0;
+      uint32_t phase = 0;
+      long armed = 0;
+      const uint32_t tx = static_cast<uint32_t>(g.a_rows * kBlockK) + plan.b_bytes;
+      bool ok = true;
+      for (int u = first; u < num_tiles && ok; u += step) {
+        const Tile t = tile_at<GROUPED>(g, kTileRows, row_start, tile_start, u);
+        const int m0 = t.m0 + static_cast<int>(rank) * kBlockM;
+        const int n0 = t.n0 + static_cast<int>(rank) * (PAIR ? g.bn / 2 : 0);
+        for (int kb = 0; kb < g.kblocks; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, wctx, kStatusTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          if (!ctl.starve) {
+            // A pair credits both CTAs' bytes to the leader's barrier.
+            if (leader) {
+              mbar_arrive_expect_tx(&full[stage], (PAIR ? 2u : 1u) * tx);
+              ++armed;
+            }
+            void *adst = a_ring + stage * plan.a_bytes;
+            void *bdst = b_ring + stage * plan.b_bytes;
+            if constexpr (PAIR) {
+              const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);
+              tma_load_3d_pair(adst, &tmap_a, bar, kb * kBlockK, m0, 0);
+              tma_load_3d_pair(bdst, &tmap_b, bar, kb * kBlockK, n0, t.group);
+            } else {
+              tma_load_3d(adst, &tmap_a, &full[stage], kb * kBlockK, m0, 0);
+              tma_load_3d(bdst, &tmap_b, &full[stage], kb * kBlockK, n0, t.group);
+            }
+          }
+          if (++stage == g.stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // Copies still in flight land before the CTA exits: wait for the fills
+      // armed last (the leader's barriers count both CTAs' copies).
+      for (long i = 0, n = armed < g.stages ? armed : g.stages; i < n; ++i) {
+        if (--stage < 0) {
+          stage = g.stages - 1;
+          phase ^= 1u;
+        }
+        mbar_wait(&full[stage], phase, wctx, kStatusTimeoutTeardown);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      // ---------------- MMA issuer (the leader of a pair) ----------------
+      const uint32_t idesc = idesc_s8(kTileRows, g.bn);
+      const uint64_t a_desc0 = smem_desc(smem_u32(a_ring), 16, 8 * kBlockK, Layout::kSw128);
+      const uint64_t b_desc0 = smem_desc(smem_u32(b_ring), 16, 8 * kBlockK, Layout::kSw128);
+      const uint32_t a_step = plan.a_bytes >> 4;
+      const uint32_t b_step = plan.b_bytes >> 4;
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int u = first; u < num_tiles && ok; u += step) {
+        if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, wctx, kStatusTimeoutDrain)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * g.bn);
+        uint32_t accumulate = 0;
+        for (int kb = 0; kb < g.kblocks; ++kb) {
+          if (!mbar_wait(&full[stage], phase, wctx, kStatusTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t ad = a_desc0 + stage * a_step;
+          const uint64_t bd = b_desc0 + stage * b_step;
+#pragma unroll
+          for (int k = 0; k < kBlockK / 32; ++k) {
+            if constexpr (PAIR)
+              umma_i8_pair(d_tmem, ad + 2 * k, bd + 2 * k, idesc, accumulate);
+            else
+              umma_i8(d_tmem, ad + 2 * k, bd + 2 * k, idesc, accumulate);
+            accumulate = 1;
+          }
+          commit_mma<PAIR>(&empty[stage]);
+          if (++stage == g.stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        commit_mma<PAIR>(&tfull[acc]);
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+      // Every MMA issued must finish before TMEM is released (in both CTAs).
+      commit_mma<PAIR>(drain);
+      mbar_wait(drain, 0, wctx, kStatusTimeoutTeardown);
+    } else if (lane == 0 && PAIR) {
+      mbar_wait(drain, 0, wctx, kStatusTimeoutTeardown);
+    }
+  } else {
+    // ---------------- epilogue (warps 2..9) ----------------
+    using T = typename Elem<OUT>::type;
+    if constexpr (!GROUPED) griddep_wait();
+    if (warp == 2) griddep_launch_dependents();
+    const int quarter = warp & 3;           // TMEM lane quarter this warp may access
+    const int half = (warp - 2) >> 2;       // 32-column blocks half, half + 2, ...
+    constexpr int kBlockBytes = 32 * 32 * out_bytes<OUT>();
+    constexpr int kBuffers = OUT == INT8CONV_FP32 ? 1 : 2;
+    uint8_t *staging = smem + plan.staging_off + (warp - 2) * kStageBytes;
+    float2 *table = reinterpret_cast<float2 *>(smem + plan.table_off + (warp - 2) * kTableBytes);
+    // The leader's tempty barriers, 8 bytes apart (a pair signals them remotely).
+    const uint32_t tempty_at = PAIR ? mapa_shared(smem_u32(tempty), 0) : smem_u32(tempty);
+    T *y = static_cast<T *>(g.y);
+    const T *residual = static_cast<const T *>(g.residual);
+    int acc = 0, buffer = 0;
+    uint32_t acc_phase = 0;
+    int table_n0 = -1, table_group = -1;
+    for (int u = first; u < num_tiles; u += step) {
+      const Tile t = tile_at<GROUPED>(g, kTileRows, row_start, tile_start, u);
+      const int row0 = t.m0 + static_cast<int>(rank) * kBlockM + quarter * 32;
+      const int rows = t.m_end - row0;        // rows of this warp's 32 that count (may be <= 0)
+      const bool mine = lane < rows;
+      if (t.n0 != table_n0 || t.group != table_group) {
+        __syncwarp();
+        const int64_t at = static_cast<int64_t>(t.group) * g.N;
+        for (int b = 0, c0 = 32 * half; c0 < g.bn; ++b, c0 += 64) {
+          const int c = t.n0 + c0 + lane;
+          float2 e = make_float2(0.f, 0.f);
+          if (c < g.N) {
+            e.x = g.col_scale != nullptr ? __ldg(g.col_scale + at + c) : 1.f;
+            e.y = g.bias != nullptr ? __ldg(g.bias + at + c) : 0.f;
+          }
+          table[b * 32 + lane] = e;
+        }
+        __syncwarp();
+        table_n0 = t.n0;
+        table_group = t.group;
+      }
+      float rs = 1.f;
+      if (g.row_scale != nullptr) rs = mine ? __ldg(g.row_scale + row0 + lane) : 0.f;
+      // All lanes wait; the vote keeps the warp converged for tcgen05.ld even
+      // if the wait runs out on some lanes only.
+      if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_phase, wctx, kStatusTimeoutAccum)))
+        break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                             static_cast<uint32_t>(acc * g.bn);
+      bool released = false;
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR)
+            mbar_arrive_cluster(tempty_at + 8u * static_cast<uint32_t>(acc));
+          else
+            mbar_arrive(&tempty[acc]);
+        }
+        released = true;
+      };
+      if (rows > 0) {
+        for (int b = 0, c0 = 32 * half; c0 < g.bn; ++b, c0 += 64) {
+          const int col0 = t.n0 + c0;
+          const int cols = g.N - col0;
+          if (cols <= 0) break;
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(taddr + c0, v);
+          tmem_ld_wait();
+          if (c0 + 64 >= g.bn || cols <= 64) release();   // this warp's last read of the tile
+          const float4 *tb = reinterpret_cast<const float4 *>(table + b * 32);
+          switch (g.activation) {
+            case INT8CONV_ACT_RELU:
+              finish_block<INT8CONV_ACT_RELU>(v, rs, tb);
+              break;
+            case INT8CONV_ACT_GELU:
+              finish_block<INT8CONV_ACT_GELU>(v, rs, tb);
+              break;
+            case INT8CONV_ACT_GELU_TANH:
+              finish_block<INT8CONV_ACT_GELU_TANH>(v, rs, tb);
+              break;
+            case INT8CONV_ACT_SILU:
+              finish_block<INT8CONV_ACT_SILU>(v, rs, tb);
+              break;
+            default:
+              finish_block<INT8CONV_ACT_NONE>(v, rs, tb);
+          }
+          if constexpr (!GROUPED && OUT != INT8CONV_INT8) {
+            if (residual != nullptr && mine)
+              add_residual<OUT>(v, residual + static_cast<int64_t>(row0 + lane) * g.ldr + col0,
+                                cols, g.vec_res != 0);
+          }
+          uint4 *stg = reinterpret_cast<uint4 *>(staging + buffer * kBlockBytes);
+          // The store that last read this buffer has finished reading it.
+          if (lane == 0) bulk_wait_group_read<kBuffers - 1>();
+          __syncwarp();
+          stage_row<OUT>(v, stg, lane, g.inv_out_scale);
+          const bool tma = g.tma_store != 0 && (!GROUPED || rows >= 32);
+          if (tma) fence_proxy_async_smem();
+          __syncwarp();
+          if (tma) {
+            if (lane == 0) tma_store_2d(&tmap_y, stg, col0, row0);
+          } else {
+            copy_out<OUT>(stg, y + static_cast<int64_t>(row0) * g.ldy + col0, g.ldy,
+                          rows < 32 ? rows : 32, cols < 32 ? cols : 32, g.vec_store != 0, lane);
+          }
+          // One group per block (empty after copy_out), so that the wait above
+          // counts blocks; the block ends together before its buffer's next use.
+          if (lane == 0) bulk_commit_group();
+          __syncwarp();
+          buffer = buffer + 1 == kBuffers ? 0 : buffer + 1;
+        }
+      }
+      if (!released) release();   // no row or column of this tile for this warp
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+    // Stores still reading shared memory finish before the CTA exits.
+    if (lane == 0) bulk_wait_group_read_all();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  // Neither CTA of a pair leaves while the other may still touch its shared
+  // memory (remote barrier arrivals, MMA operand reads).
+  if constexpr (PAIR) cluster_sync_all();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    if constexpr (PAIR)
+      tmem_dealloc_pair(tmem_base, g.tmem_cols);
+    else
+      tmem_dealloc(tmem_base, g.tmem_cols);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+// Tile choice of one launch.
+struct TileChoice {
+  bool pair;
+  int bn;
+};
+
+// The candidate with the least estimated time.  Per 128 bytes of k a CTA's
+// tensor core needs 2 * bn cycles (128 x bn x 32 bytes in bn / 2 cycles; a pair
+// 256 x bn in the same), and its loads (a_rows rows of A and its share of B,
+// 128 bytes each) come at about 64 bytes a cycle when all SMs load; the slower
+// of both counts, times the waves of tiles over the SMs, plus a per-tile cost
+// (pipeline fill and the last epilogue).
+TileChoice choose_tile(int64_t row_tiles128, int64_t row_tiles256, int64_t n, int kblocks,
+                       int a_rows, int sms) {
+  TileChoice best{false, 128};
+  double best_cost = 1e300;
+  auto consider = [&](bool pair, int bn) {
+    const int64_t n_tiles = (n + bn - 1) / bn;
+    const int64_t tiles = (pair ? row_tiles256 : row_tiles128) * n_tiles;
+    const int64_t slots = pair ? sms / 2 : sms;
+    const double waves = static_cast<double>((tiles + slots - 1) / slots);
+    const double mma = 2.0 * bn;
+    const double load = 2.0 * ((pair ? kBlockM : a_rows) + (pair ? bn / 2 : bn));
+    const double cost = waves * (kblocks * (mma > load ? mma : load) + 4.0 * bn) + 1500.0;
+    if (cost < best_cost * 0.999) {
+      best_cost = cost;
+      best = TileChoice{pair, bn};
+    }
+  };
+  if (a_rows == kBlockM && pairing_mode() != 1) {
+    consider(true, 256);
+    consider(true, 128);
+    if (pairing_mode() == 2) return best;
+  }
+  const int widths[] = {256, 128, 64, 32};
+  for (int bn : widths) consider(false, bn);
+  return best;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaDriverEntryPointQueryResult q;
+    void *p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// int8 operand [outer][rows][k]: boxes of 128 bytes of k x `box_rows` rows.
+bool operand_map(CUtensorMap *map, const int8_t *p, int64_t k, int64_t rows, int64_t ld,
+                 int64_t outer, int64_t outer_stride, int box_rows) {
+  const auto encode = encode_tiled();
+  if (encode == nullptr) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)k, (cuuint64_t)rows, (cuuint64_t)outer};
+  cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)outer_stride};
+  cuuint32_t box[3] = {kBlockK, (cuuint32_t)box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<int8_t *>(p), dims, strides, box,
+                estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Output [M][N], boxes of 32 x 32 elements, swizzled over the box's row.
+bool result_map(CUtensorMap *map, void *y, int dtype, int64_t m, int64_t n, int64_t ldy) {
+  const auto encode = encode_tiled();
+  if (encode == nullptr) return false;
+  const int size = dtype_bytes(dtype);
+  cuuint64_t dims[2] = {(cuuint64_t)n, (cuuint64_t)m};
+  cuuint64_t strides[1] = {(cuuint64_t)ldy * size};
+  cuuint32_t box[2] = {32, 32};
+  cuuint32_t estr[2] = {1, 1};
+  // Elements are moved, not computed with: unsigned types of the same size.
+  const CUtensorMapDataType type = size == 4   ? CU_TENSOR_MAP_DATA_TYPE_UINT32
+                                   : size == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  const CUtensorMapSwizzle swizzle = size == 4   ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : size == 2 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                 : CU_TENSOR_MAP_SWIZZLE_32B;
+  return encode(map, type, 2, y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool PAIR, bool GROUPED>
+const void *kernel_for(int dtype) {
+  switch (dtype) {
+    case INT8CONV_BF16:
+      return reinterpret_cast<const void *>(&matmul_kernel<PAIR, GROUPED, INT8CONV_BF16>);
+    case INT8CONV_FP16:
+      return reinterpret_cast<const void *>(&matmul_kernel<PAIR, GROUPED, INT8CONV_FP16>);
+    case INT8CONV_FP32:
+      return reinterpret_cast<const void *>(&matmul_kernel<PAIR, GROUPED, INT8CONV_FP32>);
+    default:
+      return reinterpret_cast<const void *>(&matmul_kernel<PAIR, GROUPED, INT8CONV_INT8>);
+  }
+}
+
+bool aligned(const void *p, int64_t bytes) {
+  return (reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes)) == 0;
+}
+
+}  // namespace
+
+int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, const int8_t *b,
+                                   int64_t group_stride, const int32_t *offsets, int32_t groups,
+                                   void *y, cudaStream_t stream) {
+  const bool grouped = groups > 0;
+  const int sms = device_info().sm_count;
+  const int size = dtype_bytes(d.y_dtype);
+  MatmulGeom g{};
+  g.M = static_cast<int32_t>(d.m);
+  g.N = static_cast<int32_t>(d.n);
+  g.kblocks = static_cast<int32_t>((d.k + kBlockK - 1) / kBlockK);
+  g.a_rows = 8;
+  while (g.a_rows < kBlockM && g.a_rows < d.m) g.a_rows *= 2;
+  // Row tiles: exact for a plain product; grouped, those of experts that share
+  // the rows evenly (the host does not know the offsets).
+  int64_t tiles128 = (d.m + 127) / 128, tiles256 = (d.m + 255) / 256;
+  if (grouped) {
+    const int64_t active = groups < d.m ? groups : d.m;
+    const int64_t each = (d.m + active - 1) / active;
+    tiles128 = active * ((each + 127) / 128);
+    tiles256 = active * ((each + 255) / 256);
+  }
+  const TileChoice c = choose_tile(tiles128, tiles256, d.n, g.kblocks, g.a_rows, sms);
+  g.bn = c.bn;
+  const int tile_rows = c.pair ? 2 * kBlockM : kBlockM;
+  g.n_tiles = static_cast<int32_t>((d.n + g.bn - 1) / g.bn);
+  // At most this many row tiles: a group adds at most one partly filled tile.
+  const int64_t m_tiles =
+      grouped ? d.m / tile_rows + (groups < d.m ? groups : d.m) : (d.m + tile_rows - 1) / tile_rows;
+  if (m_tiles * g.n_tiles >= (int64_t(1) << 30)) return INT8CONV_BAD_ARGUMENT;
+  g.m_tiles = static_cast<int32_t>(m_tiles);
+  g.band = 8;
+  g.tmem_cols = 2 * g.bn < 32 ? 32 : 2 * g.bn;
+  const int b_rows = c.pair ? g.bn / 2 : g.bn;
+  g.stages = kMaxStages;
+  while (g.stages > 2 &&
+         matmul_smem(b_rows, g.stages, groups).total > static_cast<uint32_t>(kMaxSmem))
+    --g.stages;
+  g.vec_store = (d.ldy * size) % 16 == 0 && aligned(y, 16);
+  // A TMA store clips the last column in units of 16 bytes, so a row that ends
+  // inside one (in a wider pitch) is stored without it.
+  g.tma_store = g.vec_store && (d.n * size) % 16 == 0;
+  g.vec_res = d.residual != nullptr && (d.ldr * size) % 16 == 0 && aligned(d.residual, 16);
+  g.activation = d.activation;
+  g.groups = groups;
+  g.inv_out_scale = d.y_dtype == INT8CONV_INT8 ? 1.0f / d.out_scale : 1.0f;
+  g.ldy = d.ldy;
+  g.ldr = d.ldr;
+  g.row_scale = d.row_scale;
+  g.col_scale = d.col_scale;
+  g.bias = d.bias;
+  g.residual = d.residual;
+  g.y = y;
+  g.offsets = offsets;
+
+  CUtensorMap tmap_a, tmap_b, tmap_y{};
+  if (!operand_map(&tmap_a, a, d.k, d.m, d.lda, 1, d.lda, g.a_rows) ||
+      !operand_map(&tmap_b, b, d.k, d.n, d.ldb, grouped ? groups : 1,
+                   groups > 1 ? group_stride : d.ldb, b_rows))
+    return INT8CONV_CUDA_ERROR;
+  if (g.tma_store && !result_map(&tmap_y, y, d.y_dtype, d.m, d.n, d.ldy)) return INT8CONV_CUDA_ERROR;
+
+  LaunchPlan plan;
+  plan.func = c.pair ? (grouped ? kernel_for<true, true>(d.y_dtype) : kernel_for<true, false>(d.y_dtype))
+                     : (grouped ? kernel_for<false, true>(d.y_dtype) : kernel_for<false, false>(d.y_dtype));
+  plan.smem = matmul_smem(b_rows, g.stages, groups).total;
+  // At least half an SM's shared memory: one CTA per SM, so that none waits
+  // for another's TMEM columns.
+  const uint32_t floor_bytes = kMaxSmem / 2 + 1024;
+  if (plan.smem < floor_bytes) plan.smem = floor_bytes;
+  if (!ensure_smem_attr(plan.func, static_cast<int>(plan.smem))) return INT8CONV_CUDA_ERROR;
+  plan.cluster = c.pair ? 2 : 1;
+  const int64_t tiles = m_tiles * g.n_tiles;
+  const int64_t slots = c.pair ? sms / 2 : sms;
+  plan.grid = dim3(static_cast<unsigned>((tiles < slots ? tiles : slots) * plan.cluster));
+  plan.block = dim3(kThreads);
+  plan_args(plan, tmap_a, tmap_b, tmap_y, g, run_ctl());
+  return launch_plan(plan, stream);
+}
+
+}  // namespace i8c
