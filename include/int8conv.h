@@ -203,6 +203,7 @@ typedef enum int8conv_activation {
 #define INT8CONV_MAX_PRODUCT_K 131071 /* |int8|^2 * k stays within int32 */
 #define INT8CONV_MAX_GROUPS 1024
 #define INT8CONV_MAX_NORM_CHANNELS 8192
+#define INT8CONV_MAX_NORM_GROUPS 4096
 
 /* One matrix product with its epilogue:
  *   acc[i,j] = sum_k a[i,k] * b[j,k]                       exact, int32
@@ -275,7 +276,8 @@ int8conv_status int8conv_launch_quantize_rows(int64_t m, int64_t k, int32_t x_dt
  * convolution launch wrote; scale is then what one step of channel c is
  * worth), y BF16, FP16, FP32 or INT8 (with out_scale as for the products).
  * Positions are ldx / ldy elements apart (>= channels), images pixels * ldx /
- * pixels * ldy.  channels % groups == 0, channels <= INT8CONV_MAX_NORM_CHANNELS.
+ * pixels * ldy.  channels % groups == 0, channels <= INT8CONV_MAX_NORM_CHANNELS,
+ * groups <= INT8CONV_MAX_NORM_GROUPS.
  * y may be x itself where types and pitches are equal.  Statistics are held in
  * fp32 as (mean, squared deviations) pairs, joined in a fixed order. */
 typedef struct int8conv_group_norm {

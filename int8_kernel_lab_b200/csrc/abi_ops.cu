@@ -54,7 +54,7 @@ int8conv_status check_norm(const int8conv_group_norm *d) {
   if (d->n < 0 || d->pixels < 0 || d->n > kMaxRows || d->pixels > kMaxRows)
     return INT8CONV_BAD_ARGUMENT;
   if (d->channels < 1 || d->channels > INT8CONV_MAX_NORM_CHANNELS || d->groups < 1 ||
-      d->channels % d->groups != 0)
+      d->groups > INT8CONV_MAX_NORM_GROUPS || d->channels % d->groups != 0)
     return INT8CONV_BAD_ARGUMENT;
   if (d->ldx < d->channels || d->ldy < d->channels || d->ldx >= kMaxPitch || d->ldy >= kMaxPitch)
     return INT8CONV_BAD_ARGUMENT;

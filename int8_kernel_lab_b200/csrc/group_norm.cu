@@ -1,18 +1,22 @@
 // group_norm.cu - group norm with an activation, channels last:
 //   v = x[i,p,c] * scale[c];  y = act((v - mean_g) * rsqrt(var_g + eps) * gamma[c] + beta[c])
 //
-// The statistics of a group run over all pixels, so x is needed twice.
-// Kernel 1 takes a chunk of an image's pixels to one (mean, squared
-// deviations) pair per group; kernel 2 joins an image's pairs and writes y,
-// reading x again (from L2, where it still is for all but the largest
-// tensors).
+// The statistics of a group run over all pixels of an image, so every value is
+// needed twice.  Two forms:
+//   one kernel   a thread-block cluster of 1 to 8 CTAs holds an image: each CTA
+//                takes a span of pixels, keeps as much of it as fits in shared
+//                memory, and the CTAs exchange their groups' partial statistics
+//                through distributed shared memory.  DRAM sees x once.
+//   two kernels  for few large images, whose clusters would leave SMs idle:
+//                statistics of pixel chunks to scratch, then the norm, reading
+//                x again (from L2 while it fits there).
 //
-// A thread owns one vector of VEC channels and walks down the pixels: 16-byte
-// loads, a warp reads whole lines, and the channel's constants stay in
-// registers.  Its sums are taken relative to the first value it saw (no
-// cancellation for a large mean), turned into (count, mean, squares) and
-// joined pairwise, threads to channels, channels to groups, chunks to images,
-// always in the same order: the result does not depend on timing.
+// A thread owns one vector of 8 channels and walks down the pixels: 16-byte
+// loads, a warp reads whole lines.  Sums are taken relative to the span's first
+// pixel (no cancellation for a large mean) in fp32, in the input's own units:
+// the channel scale is applied to the channel's mean and squares afterwards.
+// Threads, channels, CTAs and chunks are joined in a fixed order, so the result
+// does not depend on timing.
 #include <cuda_runtime.h>
 #include <math.h>
 
@@ -24,64 +28,107 @@ namespace i8c {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+// Shared memory of a CTA that leaves room for another on its SM (228 KB, of
+// which each CTA takes 1 KB for itself): one loads while the other reduces or
+// stores.
+constexpr uint32_t kHalfSmem = 113 * 1024;
 
 struct NormArgs {
   const void *x;
   void *y;
   const float *scale, *gamma, *beta;
-  float2 *partial;       // [n][chunks][groups] (mean, squared deviations)
+  float2 *partial;       // two kernels: [n][groups][spans] (mean, squared deviations)
   int64_t ldx, ldy;
-  int64_t pixels;
+  int32_t pixels;
   int32_t channels, groups, per_group;
-  int32_t chunks;        // chunks of an image in kernel 1
-  int64_t chunk_pixels;  // pixels of a chunk (the last may hold fewer)
-  int32_t apply_chunks;  // chunks of an image in kernel 2
-  int64_t apply_pixels;
+  int32_t spans;         // spans of an image: CTAs of its cluster, or chunks
+  int32_t span_pixels;   // pixels of a span (the last ones may hold fewer, or none)
+  int32_t keep;          // vectors each thread keeps in shared memory
   float eps, inv_out_scale;
   int32_t activation;
 };
 
-struct Moments {
-  float n, mean, sq;
+// Shared memory, in this order: kept vectors, the threads' sums, three values
+// of each channel, the CTA's group statistics, the image's.
+struct NormSmem {
+  uint32_t cell_off, channel_off, part_off, stat_off, total;
 };
 
-__device__ __forceinline__ Moments join(const Moments &a, const Moments &b) {
-  const float n = a.n + b.n;
-  if (n == 0.f) return a;
-  const float w = b.n / n;
-  const float d = b.mean - a.mean;
-  return Moments{n, a.mean + d * w, a.sq + b.sq + d * d * a.n * w};
+__host__ __device__ inline NormSmem norm_smem(int vec, int raw_bytes, int channels, int groups,
+                                              int keep) {
+  NormSmem p;
+  p.cell_off = static_cast<uint32_t>(keep) * kThreads * vec * raw_bytes;
+  p.channel_off = p.cell_off + kThreads * vec * sizeof(float);
+  const uint32_t padded = (channels + 3) & ~3u;   // each array starts 16-byte aligned
+  p.part_off = p.channel_off + 3 * padded * sizeof(float);
+  p.stat_off = p.part_off + groups * sizeof(float2);
+  p.total = p.stat_off + groups * sizeof(float2);
+  return p;
 }
 
-__device__ __forceinline__ Moments join_warp(Moments m) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    Moments o;
-    o.n = __shfl_down_sync(0xffffffffu, m.n, d);
-    o.mean = __shfl_down_sync(0xffffffffu, m.mean, d);
-    o.sq = __shfl_down_sync(0xffffffffu, m.sq, d);
-    m = join(m, o);
+// Three arrays over the channels.  Statistics: the shift, then the mean; sums,
+// then squares.  Norm: y = act((x - m) * w + b), m in the input's own units.
+struct Channels {
+  float *m, *w, *b;
+  __device__ __forceinline__ Channels(uint8_t *smem, const NormSmem &plan, int channels) {
+    const int padded = (channels + 3) & ~3;
+    m = reinterpret_cast<float *>(smem + plan.channel_off);
+    w = m + padded;
+    b = w + padded;
   }
-  return m;
-}
+};
 
+// scale, gamma and beta of one channel.
+struct Params {
+  float scale, gamma, beta;
+  __device__ __forceinline__ Params(const NormArgs &a, int c) {
+    const bool in = c < a.channels;
+    scale = in && a.scale != nullptr ? __ldg(a.scale + c) : 1.f;
+    gamma = in && a.gamma != nullptr ? __ldg(a.gamma + c) : 1.f;
+    beta = in && a.beta != nullptr ? __ldg(a.beta + c) : 0.f;
+  }
+};
+
+// VEC elements as they lie in memory.
 template <int DT, int VEC>
-__device__ __forceinline__ void load_vec(const typename Elem<DT>::type *p, float (&f)[VEC]) {
+struct Raw {
   using T = typename Elem<DT>::type;
-  if constexpr (VEC == 1) {
-    f[0] = Elem<DT>::load(*p);
-  } else {
-    constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  static constexpr int kWords = VEC == 1 ? 1 : VEC * static_cast<int>(sizeof(T)) / 16;
+  uint4 w[kWords];   // VEC == 1: the element alone, in w[0].x
+
+  __device__ __forceinline__ void load(const T *p) {
+    if constexpr (VEC == 1) {
+      *reinterpret_cast<T *>(&w[0].x) = *p;
+    } else {
 #pragma unroll
-    for (int j = 0; j < VEC / kPer; ++j) {
-      const uint4 raw = reinterpret_cast<const uint4 *>(p)[j];
-      const T *e = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-      for (int t = 0; t < kPer; ++t) f[j * kPer + t] = Elem<DT>::load(e[t]);
+      for (int j = 0; j < kWords; ++j) w[j] = reinterpret_cast<const uint4 *>(p)[j];
     }
   }
-}
+  __device__ __forceinline__ float get(int j) const {
+    return Elem<DT>::load(reinterpret_cast<const T *>(&w[0])[j]);
+  }
+  // A kept vector, word by word at `slot` + threadIdx.x, so that a warp's
+  // accesses are contiguous.  VEC == 8 only.
+  __device__ __forceinline__ void keep(uint4 *slot) const {
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) slot[j * kThreads + threadIdx.x] = w[j];
+  }
+  __device__ __forceinline__ void kept(const uint4 *slot) {
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) w[j] = slot[j * kThreads + threadIdx.x];
+  }
+  // Elements j and j + 1 (j even) as an fp32 pair.
+  __device__ __forceinline__ uint64_t pair(int j) const {
+    if constexpr (DT == INT8CONV_BF16) {
+      const uint32_t u = reinterpret_cast<const uint32_t *>(w)[j >> 1];
+      return f2_pack(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    } else {
+      return f2_pack(get(j), get(j + 1));
+    }
+  }
+};
 
 template <int OUT, int VEC>
 __device__ __forceinline__ void store_vec(typename Elem<OUT>::type *p, const float (&f)[VEC]) {
@@ -103,237 +150,519 @@ __device__ __forceinline__ void store_vec(typename Elem<OUT>::type *p, const flo
   }
 }
 
-// Kernel 1.  Dynamic shared memory: kThreads * VEC (mean, squares) pairs.
+template <int VEC>
+__device__ __forceinline__ void put_vec(float *p, const float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    *p = v[0];
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC / 4; ++j)
+      reinterpret_cast<float4 *>(p)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void get_vec(const float *p, float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    v[0] = *p;
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC / 4; ++j) {
+      const float4 t = reinterpret_cast<const float4 *>(p)[j];
+      v[4 * j] = t.x;
+      v[4 * j + 1] = t.y;
+      v[4 * j + 2] = t.z;
+      v[4 * j + 3] = t.w;
+    }
+  }
+}
+
+// How the CTA's threads share a tile of at most kThreads columns (vectors of
+// VEC channels): `lanes` threads down each column.
+struct Columns {
+  int width, lanes, col, part;
+  __device__ __forceinline__ Columns(int cols, int col0) {
+    width = cols - col0 < kThreads ? cols - col0 : kThreads;
+    lanes = kThreads / width;
+    col = static_cast<int>(threadIdx.x) % width;
+    part = static_cast<int>(threadIdx.x) / width;
+  }
+};
+
+// Pixels read before the first of them is used.
 template <int DT, int VEC>
-__global__ void __launch_bounds__(kThreads) norm_stats_kernel(const NormArgs a) {
-  extern __shared__ float2 cell[];   // [row of threads][channel of the column tile]
+constexpr int batch() {
+  return VEC == 1 ? 8 : (sizeof(typename Elem<DT>::type) == 2 ? 4 : 2);
+}
+
+__device__ __forceinline__ int rows_of(const NormArgs &a, int span) {
+  const int left = a.pixels - span * a.span_pixels;
+  return left <= 0 ? 0 : (left < a.span_pixels ? left : a.span_pixels);
+}
+
+// (mean, squared deviations) of every group over pixels [0, rows) of x, this
+// CTA's span, into part[].  `mine`: the parameters of channel threadIdx.x.
+template <int DT, int VEC>
+__device__ __forceinline__ void span_stats(const NormArgs &a, const typename Elem<DT>::type *x,
+                                           int rows, uint8_t *area, float *cell,
+                                           const Channels &ch, const Params &mine, float2 *part) {
   using T = typename Elem<DT>::type;
-  griddep_wait();
-  griddep_launch_dependents();
-  const int64_t image = blockIdx.x / a.chunks;
-  const int chunk = static_cast<int>(blockIdx.x % a.chunks);
-  const int64_t begin = chunk * a.chunk_pixels;
-  const int64_t end = begin + a.chunk_pixels < a.pixels ? begin + a.chunk_pixels : a.pixels;
-  const T *x = static_cast<const T *>(a.x) + image * a.pixels * a.ldx;
+  constexpr int kBatch = batch<DT, VEC>();
   const int cols = a.channels / VEC;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // (mean, squares) of every channel of the chunk.
-  float2 *channel = cell + kThreads * VEC;   // [channels]
+  uint4 *slot = reinterpret_cast<uint4 *>(area);
+  int kept = a.keep;   // full batches go to shared memory until this many vectors lie there
   for (int col0 = 0; col0 < cols; col0 += kThreads) {
-    const int width = cols - col0 < kThreads ? cols - col0 : kThreads;
-    const int lanes = kThreads / width;      // threads that share a column
-    const int col = threadIdx.x % width;
-    const int part = threadIdx.x / width;
-    if (part < lanes) {
-      const int c0 = (col0 + col) * VEC;
-      float s[VEC], x0[VEC], s1[VEC], s2[VEC];
+    const Columns k(cols, col0);
+    const bool active = k.part < k.lanes;
+    float x0[VEC], s1[VEC], s2[VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        s[j] = a.scale != nullptr ? __ldg(a.scale + c0 + j) : 1.f;
-        x0[j] = s1[j] = s2[j] = 0.f;
-      }
-      int64_t p = begin + part;
-      float f[VEC];
-      if (p < end) {
-        load_vec<DT, VEC>(x + p * a.ldx + c0, f);
+    for (int j = 0; j < VEC; ++j) x0[j] = s1[j] = s2[j] = 0.f;
+    if (active && rows > 0) {
+      const T *at = x + (col0 + k.col) * VEC;
+      Raw<DT, VEC> shift;
+      shift.load(at);
+      at += k.part * a.ldx;
+      const int64_t step = k.lanes * a.ldx;
+      int left = k.part < rows ? (rows - k.part - 1) / k.lanes + 1 : 0;   // this thread's pixels
+      auto add = [&](const Raw<DT, VEC> &r) {
+        if constexpr (VEC == 1) {
+          const float d = r.get(0) - x0[0];
+          s1[0] += d;
+          s2[0] = fmaf(d, d, s2[0]);
+        } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) x0[j] = f[j] * s[j];
-        p += lanes;
-      }
-#pragma unroll 4
-      for (; p < end; p += lanes) {
-        load_vec<DT, VEC>(x + p * a.ldx + c0, f);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float d = fmaf(f[j], s[j], -x0[j]);
-          s1[j] += d;
-          s2[j] = fmaf(d, d, s2[j]);
+          for (int j = 0; j < VEC; j += 2) {
+            const uint64_t d = f2_add(r.pair(j), f2_pack(-x0[j], -x0[j + 1]));
+            f2_unpack(f2_add(f2_pack(s1[j], s1[j + 1]), d), s1[j], s1[j + 1]);
+            f2_unpack(f2_fma(d, d, f2_pack(s2[j], s2[j + 1])), s2[j], s2[j + 1]);
+          }
         }
-      }
-      const int64_t count = begin + part < end ? (end - begin - part + lanes - 1) / lanes : 0;
-      const float inv = count > 0 ? 1.f / static_cast<float>(count) : 0.f;
+      };
+      bool first = true;
+#pragma unroll 1
+      for (; left >= kBatch; left -= kBatch) {
+        Raw<DT, VEC> r[kBatch];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float d = s1[j] * inv;
-        const float sq = s2[j] - s1[j] * d;
-        cell[part * width * VEC + col * VEC + j] = make_float2(x0[j] + d, sq > 0.f || sq != sq ? sq : 0.f);
-      }
-    }
-    __syncthreads();
-    for (int c = threadIdx.x; c < width * VEC; c += kThreads) {
-      Moments m{0.f, 0.f, 0.f};
-      for (int q = 0; q < lanes; ++q) {
-        const int64_t count = begin + q < end ? (end - begin - q + lanes - 1) / lanes : 0;
-        const float2 e = cell[q * width * VEC + c];
-        m = join(m, Moments{static_cast<float>(count), e.x, e.y});
-      }
-      channel[col0 * VEC + c] = make_float2(m.mean, m.sq);
-    }
-    __syncthreads();
-  }
-  const float rows = static_cast<float>(end - begin);
-  for (int g = warp; g < a.groups; g += kThreads / 32) {
-    Moments m{0.f, 0.f, 0.f};
-    for (int c = lane; c < a.per_group; c += 32) {
-      const float2 e = channel[g * a.per_group + c];
-      m = join(m, Moments{rows, e.x, e.y});
-    }
-    m = join_warp(m);
-    if (lane == 0)
-      a.partial[(image * a.chunks + chunk) * a.groups + g] =
-          make_float2(m.mean, m.sq);
-  }
-}
-
-// Rows [begin, end) of one image through the norm; mean[] and rstd[] of its
-// groups in shared memory.
-template <int DT, int OUT, int VEC, int ACT>
-__device__ __forceinline__ void apply_rows(const NormArgs &a, const typename Elem<DT>::type *x,
-                                           typename Elem<OUT>::type *y, int64_t begin, int64_t end,
-                                           const float *mean, const float *rstd) {
-  const int cols = a.channels / VEC;
-  for (int col0 = 0; col0 < cols; col0 += kThreads) {
-    const int width = cols - col0 < kThreads ? cols - col0 : kThreads;
-    const int lanes = kThreads / width;
-    const int col = threadIdx.x % width;
-    const int part = threadIdx.x / width;
-    if (part >= lanes) continue;
-    const int c0 = (col0 + col) * VEC;
-    float s[VEC], m[VEC], w[VEC], b[VEC];
+        for (int u = 0; u < kBatch; ++u, at += step) r[u].load(at);
+        if (first) {   // the shift was on its way together with the first batch
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const int g = (c0 + j) / a.per_group;
-      s[j] = a.scale != nullptr ? __ldg(a.scale + c0 + j) : 1.f;
-      m[j] = mean[g];
-      w[j] = rstd[g] * (a.gamma != nullptr ? __ldg(a.gamma + c0 + j) : 1.f);
-      b[j] = a.beta != nullptr ? __ldg(a.beta + c0 + j) : 0.f;
-    }
-    auto finish = [&](float (&f)[VEC], int64_t p) {
+          for (int j = 0; j < VEC; ++j) x0[j] = shift.get(j);
+          first = false;
+        }
+        if constexpr (VEC > 1) {
+          if (kept > 0) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        f[j] = activate<ACT>(fmaf(fmaf(f[j], s[j], -m[j]), w[j], b[j]));
-        if constexpr (OUT == INT8CONV_INT8) f[j] *= a.inv_out_scale;
+            for (int u = 0; u < kBatch; ++u, slot += Raw<DT, VEC>::kWords * kThreads)
+              r[u].keep(slot);
+            kept -= kBatch;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) add(r[u]);
       }
-      store_vec<OUT, VEC>(y + p * a.ldy + c0, f);
+      if (first) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x0[j] = shift.get(j);
+      }
+#pragma unroll 1
+      for (; left > 0; --left, at += step) {
+        Raw<DT, VEC> r;
+        r.load(at);
+        add(r);
+      }
+    }
+    // The sums of a column's threads, first all of one kind, then of the other
+    // through the same memory: cell[thread of the column][channel].
+    const int wide = k.width * VEC, c0 = col0 * VEC;
+    const float inv = 1.f / static_cast<float>(rows > 0 ? rows : 1);
+    auto gather = [&](const float (&v)[VEC]) {
+      if (active) put_vec<VEC>(cell + k.part * wide + k.col * VEC, v);
+      __syncthreads();
     };
-    // Several pixels are read before the first is written: y may be x, so the
-    // compiler may not move a load above a store itself.
-    constexpr int kBatch = 4;
-    int64_t p = begin + part;
-    for (; p + (kBatch - 1) * lanes < end; p += kBatch * lanes) {
-      float f[kBatch][VEC];
+    auto total = [&](int i) {
+      float t = 0.f;
+#pragma unroll 4
+      for (int q = 0; q < k.lanes; ++q) t += cell[q * wide + i];
+      return t;
+    };
+    if (k.part == 0) {
+      // The threads without a pixel hold no shift; the first has one.
+      if (rows > 0) {
+        put_vec<VEC>(ch.m + c0 + k.col * VEC, x0);
+      } else {
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) load_vec<DT, VEC>(x + (p + u * lanes) * a.ldx + c0, f[u]);
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) finish(f[u], p + u * lanes);
+        for (int j = 0; j < VEC; ++j) ch.m[c0 + k.col * VEC + j] = 0.f;
+      }
     }
-    for (; p < end; p += lanes) {
-      float f[VEC];
-      load_vec<DT, VEC>(x + p * a.ldx + c0, f);
-      finish(f, p);
+    gather(s1);
+#pragma unroll 1
+    for (int i = threadIdx.x; i < wide; i += kThreads) ch.w[c0 + i] = total(i);
+    __syncthreads();
+    gather(s2);
+#pragma unroll 1
+    for (int i = threadIdx.x; i < wide; i += kThreads) {
+      const int c = c0 + i;
+      const float s = c == static_cast<int>(threadIdx.x) ? mine.scale : Params(a, c).scale;
+      const float sum = ch.w[c];
+      const float d = sum * inv;
+      const float sq = total(i) - sum * d;     // not below zero; NaN stays NaN
+      ch.m[c] = (ch.m[c] + d) * s;
+      ch.w[c] = (sq < 0.f ? 0.f : sq) * s * s;
     }
+    __syncthreads();
+  }
+  // Channels of a group all hold `rows` values: the mean of means (relative to
+  // the first, so that a large mean costs no bits), and the squares plus `rows`
+  // times the means' squared deviations.  2 to 32 lanes share a group.
+  const int lane = threadIdx.x & 31;
+  int share = 2;
+  while (share < 32 && share < a.per_group) share *= 2;
+  const int sub = lane & (share - 1);
+  const float inv = 1.f / static_cast<float>(a.per_group);
+  const float n = static_cast<float>(rows);
+#pragma unroll 1
+  for (int g0 = 0; g0 < a.groups; g0 += kThreads / share) {
+    const int g = g0 + static_cast<int>(threadIdx.x) / share;
+    const int first = (g < a.groups ? g : 0) * a.per_group;
+    const float ref = ch.m[first];
+    float mean = 0.f, sq = 0.f;
+#pragma unroll 1
+    for (int c = sub; c < a.per_group; c += share) mean += ch.m[first + c] - ref;
+#pragma unroll 1
+    for (int d = share >> 1; d > 0; d >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, d);
+    mean = fmaf(mean, inv, ref);
+#pragma unroll 1
+    for (int c = sub; c < a.per_group; c += share) {
+      const float d = ch.m[first + c] - mean;
+      sq += fmaf(d * n, d, ch.w[first + c]);
+    }
+#pragma unroll 1
+    for (int d = share >> 1; d > 0; d >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, d);
+    if (sub == 0 && g < a.groups) part[g] = make_float2(mean, sq);
   }
 }
 
-template <int DT, int OUT, int VEC>
-__device__ __forceinline__ void apply_rows_act(const NormArgs &a, const typename Elem<DT>::type *x,
-                                               typename Elem<OUT>::type *y, int64_t begin,
-                                               int64_t end, const float *mean, const float *rstd) {
-  switch (a.activation) {
-    case INT8CONV_ACT_RELU:
-      apply_rows<DT, OUT, VEC, INT8CONV_ACT_RELU>(a, x, y, begin, end, mean, rstd);
-      break;
-    case INT8CONV_ACT_GELU:
-      apply_rows<DT, OUT, VEC, INT8CONV_ACT_GELU>(a, x, y, begin, end, mean, rstd);
-      break;
-    case INT8CONV_ACT_GELU_TANH:
-      apply_rows<DT, OUT, VEC, INT8CONV_ACT_GELU_TANH>(a, x, y, begin, end, mean, rstd);
-      break;
-    case INT8CONV_ACT_SILU:
-      apply_rows<DT, OUT, VEC, INT8CONV_ACT_SILU>(a, x, y, begin, end, mean, rstd);
-      break;
-    default:
-      apply_rows<DT, OUT, VEC, INT8CONV_ACT_NONE>(a, x, y, begin, end, mean, rstd);
-  }
-}
-
-// Kernel 2.  Dynamic shared memory: mean[groups], rstd[groups].
-template <int DT, int OUT, int VEC>
-__global__ void __launch_bounds__(kThreads) norm_apply_kernel(const NormArgs a) {
-  extern __shared__ float stats[];
-  using T = typename Elem<DT>::type;
-  using O = typename Elem<OUT>::type;
-  float *mean = stats, *rstd = stats + a.groups;
-  griddep_wait();
-  griddep_launch_dependents();
-  const int64_t image = blockIdx.x / a.apply_chunks;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int g = warp; g < a.groups; g += kThreads / 32) {
-    Moments m{0.f, 0.f, 0.f};
-    for (int k = lane; k < a.chunks; k += 32) {
-      const int64_t begin = k * a.chunk_pixels;
-      const int64_t rows = begin + a.chunk_pixels < a.pixels ? a.chunk_pixels : a.pixels - begin;
-      const float2 e = a.partial[(image * a.chunks + k) * a.groups + g];
-      m = join(m, Moments{static_cast<float>(rows) * a.per_group, e.x, e.y});
-    }
-    m = join_warp(m);
-    if (lane == 0) {
-      mean[g] = m.mean;
-      rstd[g] = rsqrtf(m.sq / m.n + a.eps);
+// The channels' constants of y = act((x - m) * w + b) from the image's
+// statistics stat[g] = (mean, 1 / deviation).
+__device__ __forceinline__ void channel_constants(const NormArgs &a, const float2 *stat,
+                                                  const Channels &ch, const Params &mine) {
+#pragma unroll 1
+  for (int c = threadIdx.x; c < a.channels; c += kThreads) {
+    const Params p = c == static_cast<int>(threadIdx.x) ? mine : Params(a, c);
+    const float2 t = stat[c / a.per_group];
+    const float w = t.y * p.gamma;
+    if (p.scale == 0.f) {     // a channel that is zero throughout
+      ch.m[c] = 0.f;
+      ch.w[c] = 0.f;
+      ch.b[c] = fmaf(-t.x, w, p.beta);
+    } else {
+      ch.m[c] = p.scale == 1.f ? t.x : t.x / p.scale;
+      ch.w[c] = w * p.scale;
+      ch.b[c] = p.beta;
     }
   }
   __syncthreads();
-  const int64_t begin = (blockIdx.x % a.apply_chunks) * a.apply_pixels;
-  const int64_t end = begin + a.apply_pixels < a.pixels ? begin + a.apply_pixels : a.pixels;
-  const T *x = static_cast<const T *>(a.x) + image * a.pixels * a.ldx;
-  O *y = static_cast<O *>(a.y) + image * a.pixels * a.ldy;
-  apply_rows_act<DT, OUT, VEC>(a, x, y, begin, end, mean, rstd);
+}
+
+// Pixels [0, rows) of x through the norm into y.
+template <int DT, int OUT, int VEC, int ACT>
+__device__ __forceinline__ void apply_span(const NormArgs &a, const typename Elem<DT>::type *x,
+                                           typename Elem<OUT>::type *y, int rows,
+                                           const uint8_t *area, const Channels &ch) {
+  using T = typename Elem<DT>::type;
+  using O = typename Elem<OUT>::type;
+  constexpr int kBatch = batch<DT, VEC>();
+  const int cols = a.channels / VEC;
+  const uint4 *slot = reinterpret_cast<const uint4 *>(area);
+  int kept = a.keep;
+  for (int col0 = 0; col0 < cols; col0 += kThreads) {
+    const Columns k(cols, col0);
+    if (k.part >= k.lanes) continue;
+    const int c0 = (col0 + k.col) * VEC;
+    float m[VEC], w[VEC], b[VEC];
+    get_vec<VEC>(ch.m + c0, m);
+    get_vec<VEC>(ch.w + c0, w);
+    get_vec<VEC>(ch.b + c0, b);
+    const T *at = x + k.part * a.ldx + c0;
+    O *to = y + k.part * a.ldy + c0;
+    const int64_t step = k.lanes * a.ldx, to_step = k.lanes * a.ldy;
+    int left = k.part < rows ? (rows - k.part - 1) / k.lanes + 1 : 0;
+    auto finish = [&](const Raw<DT, VEC> &r) {
+      float f[VEC];
+      if constexpr (VEC == 1) {
+        f[0] = activate<ACT>(fmaf(r.get(0) - m[0], w[0], b[0]));
+        if constexpr (OUT == INT8CONV_INT8) f[0] *= a.inv_out_scale;
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+          const uint64_t d = f2_add(r.pair(j), f2_pack(-m[j], -m[j + 1]));
+          f2_unpack(f2_fma(d, f2_pack(w[j], w[j + 1]), f2_pack(b[j], b[j + 1])), f[j], f[j + 1]);
+          activate2<ACT>(f[j], f[j + 1]);
+          if constexpr (OUT == INT8CONV_INT8)
+            f2_unpack(f2_mul(f2_pack(f[j], f[j + 1]), f2_pack(a.inv_out_scale, a.inv_out_scale)),
+                      f[j], f[j + 1]);
+        }
+      }
+      store_vec<OUT, VEC>(to, f);
+      to += to_step;
+    };
+    // A batch is read before its first pixel is written: y may be x, so the
+    // compiler may not move a load above a store itself.
+#pragma unroll 1
+    for (; left >= kBatch; left -= kBatch) {
+      Raw<DT, VEC> r[kBatch];
+      bool here = false;
+      if constexpr (VEC > 1) {
+        here = kept > 0;
+        if (here) {
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u, slot += Raw<DT, VEC>::kWords * kThreads) r[u].kept(slot);
+          kept -= kBatch;
+          at += kBatch * step;
+        }
+      }
+      if (!here) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u, at += step) r[u].load(at);
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) finish(r[u]);
+    }
+#pragma unroll 1
+    for (; left > 0; --left, at += step) {
+      Raw<DT, VEC> r;
+      r.load(at);
+      finish(r);
+    }
+  }
+}
+
+template <int DT, int OUT, int VEC>
+__device__ __forceinline__ void apply_span_act(const NormArgs &a, const typename Elem<DT>::type *x,
+                                               typename Elem<OUT>::type *y, int rows,
+                                               const uint8_t *area, const Channels &ch) {
+  switch (a.activation) {
+    case INT8CONV_ACT_RELU:
+      apply_span<DT, OUT, VEC, INT8CONV_ACT_RELU>(a, x, y, rows, area, ch);
+      break;
+    case INT8CONV_ACT_GELU:
+      apply_span<DT, OUT, VEC, INT8CONV_ACT_GELU>(a, x, y, rows, area, ch);
+      break;
+    case INT8CONV_ACT_GELU_TANH:
+      apply_span<DT, OUT, VEC, INT8CONV_ACT_GELU_TANH>(a, x, y, rows, area, ch);
+      break;
+    case INT8CONV_ACT_SILU:
+      apply_span<DT, OUT, VEC, INT8CONV_ACT_SILU>(a, x, y, rows, area, ch);
+      break;
+    default:
+      apply_span<DT, OUT, VEC, INT8CONV_ACT_NONE>(a, x, y, rows, area, ch);
+  }
+}
+
+__device__ __forceinline__ float2 finish_stat(const NormArgs &a, float mean, float sq) {
+  const float n = static_cast<float>(a.pixels) * static_cast<float>(a.per_group);
+  return make_float2(mean, rsqrtf(sq / n + a.eps));
+}
+
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+constexpr int kMaxCluster = 8;
+
+// One kernel: the CTAs of a cluster share an image.
+template <int DT, int OUT, int VEC>
+__global__ void __launch_bounds__(kThreads, 2) norm_cluster_kernel(const NormArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  using T = typename Elem<DT>::type;
+  using O = typename Elem<OUT>::type;
+  const NormSmem plan = norm_smem(VEC, sizeof(T), a.channels, a.groups, a.keep);
+  const Channels ch(smem, plan, a.channels);
+  float2 *part = reinterpret_cast<float2 *>(smem + plan.part_off);
+  float2 *stat = reinterpret_cast<float2 *>(smem + plan.stat_off);
+  griddep_wait();
+  griddep_launch_dependents();
+  const Params mine(a, threadIdx.x);
+  const int64_t image = blockIdx.x / a.spans;
+  const int span = static_cast<int>(blockIdx.x) % a.spans;   // rank in the cluster
+  const int rows = rows_of(a, span);
+  const int64_t first = image * a.pixels + static_cast<int64_t>(span) * a.span_pixels;
+  const T *x = static_cast<const T *>(a.x) + first * a.ldx;
+  span_stats<DT, VEC>(a, x, rows, smem, reinterpret_cast<float *>(smem + plan.cell_off), ch, mine,
+                      part);
+  cluster_sync_all();
+  // 8 lanes share a group, one for each CTA of the cluster.
+  const int k = threadIdx.x & (kMaxCluster - 1);
+  const float n = k < a.spans ? static_cast<float>(rows_of(a, k)) : 0.f;
+  const float share = n / static_cast<float>(a.pixels);
+#pragma unroll 1
+  for (int g0 = 0; g0 < a.groups; g0 += kThreads / kMaxCluster) {
+    const int g = g0 + static_cast<int>(threadIdx.x) / kMaxCluster;
+    float2 e = make_float2(0.f, 0.f);
+    if (n > 0.f && g < a.groups) e = ld_cluster_f2(mapa_shared(smem_u32(part + g), k));
+    const float ref = __shfl_sync(0xffffffffu, e.x, 0, kMaxCluster);   // span 0 is never empty
+    float mean = n > 0.f ? share * (e.x - ref) : 0.f;
+#pragma unroll
+    for (int d = kMaxCluster / 2; d > 0; d >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, d);
+    mean += ref;
+    const float dev = e.x - mean;
+    float sq = n > 0.f ? fmaf(dev * n * static_cast<float>(a.per_group), dev, e.y) : 0.f;
+#pragma unroll
+    for (int d = kMaxCluster / 2; d > 0; d >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, d);
+    if (k == 0 && g < a.groups) stat[g] = finish_stat(a, mean, sq);
+  }
+  // No CTA leaves while another may still read its part; and stat[] is complete.
+  cluster_sync_all();
+  channel_constants(a, stat, ch, mine);
+  O *y = static_cast<O *>(a.y) + first * a.ldy;
+  apply_span_act<DT, OUT, VEC>(a, x, y, rows, smem, ch);
+}
+
+// Two kernels, the first: statistics of one chunk of pixels.
+template <int DT, int VEC>
+__global__ void __launch_bounds__(kThreads, 2) norm_stats_kernel(const NormArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  using T = typename Elem<DT>::type;
+  const NormSmem plan = norm_smem(VEC, sizeof(T), a.channels, a.groups, 0);
+  const Channels ch(smem, plan, a.channels);
+  float2 *part = reinterpret_cast<float2 *>(smem + plan.part_off);
+  griddep_wait();
+  griddep_launch_dependents();
+  const Params mine(a, threadIdx.x);
+  const int64_t image = blockIdx.x / a.spans;
+  const int span = static_cast<int>(blockIdx.x) % a.spans;
+  const int64_t first = image * a.pixels + static_cast<int64_t>(span) * a.span_pixels;
+  span_stats<DT, VEC>(a, static_cast<const T *>(a.x) + first * a.ldx, rows_of(a, span), smem,
+                      reinterpret_cast<float *>(smem + plan.cell_off), ch, mine, part);
+  __syncthreads();
+  for (int g = threadIdx.x; g < a.groups; g += kThreads)
+    a.partial[(image * a.groups + g) * a.spans + span] = part[g];
+}
+
+// The second: a warp joins the chunks of a group, then the chunk is normalised.
+template <int DT, int OUT, int VEC>
+__global__ void __launch_bounds__(kThreads, 2) norm_apply_kernel(const NormArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  using T = typename Elem<DT>::type;
+  using O = typename Elem<OUT>::type;
+  const NormSmem plan = norm_smem(VEC, sizeof(T), a.channels, a.groups, 0);
+  const Channels ch(smem, plan, a.channels);
+  float2 *stat = reinterpret_cast<float2 *>(smem + plan.stat_off);
+  griddep_wait();
+  griddep_launch_dependents();
+  const Params mine(a, threadIdx.x);
+  const int64_t image = blockIdx.x / a.spans;
+  const int span = static_cast<int>(blockIdx.x) % a.spans;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float inv = 1.f / static_cast<float>(a.pixels);
+  for (int g = warp; g < a.groups; g += kWarps) {
+    const float2 *e = a.partial + (image * a.groups + g) * a.spans;
+    const float ref = e[0].x;
+    float mean = 0.f, sq = 0.f;
+    for (int k = lane; k < a.spans; k += 32)
+      mean = fmaf(static_cast<float>(rows_of(a, k)) * inv, e[k].x - ref, mean);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, d);
+    mean += ref;
+    for (int k = lane; k < a.spans; k += 32) {
+      const float n = static_cast<float>(rows_of(a, k)) * static_cast<float>(a.per_group);
+      const float d = e[k].x - mean;
+      sq += fmaf(d * n, d, e[k].y);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, d);
+    if (lane == 0) stat[g] = finish_stat(a, mean, sq);
+  }
+  __syncthreads();
+  channel_constants(a, stat, ch, mine);
+  const int64_t first = image * a.pixels + static_cast<int64_t>(span) * a.span_pixels;
+  apply_span_act<DT, OUT, VEC>(a, static_cast<const T *>(a.x) + first * a.ldx,
+                               static_cast<O *>(a.y) + first * a.ldy, rows_of(a, span), smem, ch);
+}
+
+struct NormKernels {
+  const void *cluster, *stats, *apply;
+};
+
+template <int DT, int OUT, int VEC>
+NormKernels kernels_of() {
+  return NormKernels{reinterpret_cast<const void *>(&norm_cluster_kernel<DT, OUT, VEC>),
+                     reinterpret_cast<const void *>(&norm_stats_kernel<DT, VEC>),
+                     reinterpret_cast<const void *>(&norm_apply_kernel<DT, OUT, VEC>)};
 }
 
 template <int DT, int VEC>
-const void *apply_for(int out) {
+NormKernels kernels_for_out(int out) {
   switch (out) {
     case INT8CONV_BF16:
-      return reinterpret_cast<const void *>(&norm_apply_kernel<DT, INT8CONV_BF16, VEC>);
+      return kernels_of<DT, INT8CONV_BF16, VEC>();
     case INT8CONV_FP16:
-      return reinterpret_cast<const void *>(&norm_apply_kernel<DT, INT8CONV_FP16, VEC>);
+      return kernels_of<DT, INT8CONV_FP16, VEC>();
     case INT8CONV_FP32:
-      return reinterpret_cast<const void *>(&norm_apply_kernel<DT, INT8CONV_FP32, VEC>);
+      return kernels_of<DT, INT8CONV_FP32, VEC>();
     default:
-      return reinterpret_cast<const void *>(&norm_apply_kernel<DT, INT8CONV_INT8, VEC>);
+      return kernels_of<DT, INT8CONV_INT8, VEC>();
   }
 }
 
 template <int DT>
-void kernels_for(bool vec, int out, const void **stats, const void **apply) {
-  *stats = vec ? reinterpret_cast<const void *>(&norm_stats_kernel<DT, 8>)
-               : reinterpret_cast<const void *>(&norm_stats_kernel<DT, 1>);
-  *apply = vec ? apply_for<DT, 8>(out) : apply_for<DT, 1>(out);
+NormKernels kernels_for(bool vec, int out) {
+  return vec ? kernels_for_out<DT, 8>(out) : kernels_for_out<DT, 1>(out);
 }
 
-// Chunks of an image: enough CTAs for the GPU four times over all images, but
-// at least 16 KB of channels x pixels each.
-int64_t pick_chunk_pixels(const int8conv_group_norm &d) {
-  const int64_t want = (4 * 148 + d.n - 1) / d.n;
-  int64_t pixels = (d.pixels + want - 1) / want;
-  const int64_t least = (8192 + d.channels - 1) / d.channels;
-  return pixels > least ? pixels : least;
+// How a call runs: spans of an image, and whether they are one cluster.
+struct NormShape {
+  bool cluster;
+  int spans;
+  int64_t span_pixels;
+};
+
+NormShape norm_shape(const int8conv_group_norm &d) {
+  const int64_t bytes = d.pixels * d.channels * dtype_bytes(d.x_dtype);   // of one image
+  // Clusters that fill the GPU: 128 CTAs, or, with 16 MB and more to read, two
+  // for each SM (measured, us: 32 images of 196 x 512 bf16 in clusters of 1 / 4 /
+  // 8: 15.6 / 9.6 / 11.1; 64 of 3136 x 256 int32: 191 / 86 / 90).  16 CTAs never
+  // pay: at most 7 such clusters find room on the GPU at one time.
+  const int64_t want = d.n * bytes < (16 << 20) ? 128 : 256;
+  int spans = 1;
+  while (spans < kMaxCluster && d.n * spans < want && bytes > spans * int64_t(8 * 1024)) spans *= 2;
+  if (spans > d.pixels) spans = 1;
+  NormShape s{true, spans, (d.pixels + spans - 1) / spans};
+  // Few images with more than 32 KB for each CTA of such a cluster: two kernels
+  // over chunks of all images, one CTA for each SM, or two where each still has
+  // 128 KB (8 images of 4096 x 320 bf16: 19.2 us, in clusters of 8 28.4;
+  // 1 image: 9.9 and 24.6).
+  if (d.n * spans < 96 && bytes > spans * int64_t(32 * 1024)) {
+    const int64_t all = d.n * bytes > 148 * int64_t(128 * 1024) ? 296 : 148;
+    int64_t chunks = (all + d.n - 1) / d.n;
+    if (chunks > d.pixels) chunks = d.pixels;
+    s.cluster = false;
+    s.span_pixels = (d.pixels + chunks - 1) / chunks;
+    s.spans = static_cast<int>((d.pixels + s.span_pixels - 1) / s.span_pixels);
+  }
+  return s;
 }
 
 }  // namespace
 
 int64_t group_norm_blocks(const int8conv_group_norm &d) {
   if (d.n == 0 || d.pixels == 0) return 0;
-  const int64_t per = pick_chunk_pixels(d);
-  return d.n * ((d.pixels + per - 1) / per);
+  return d.n * norm_shape(d).spans;
 }
 
 size_t group_norm_workspace(const int8conv_group_norm &d) {
-  return static_cast<size_t>(group_norm_blocks(d)) * static_cast<size_t>(d.groups) * sizeof(float2);
+  if (d.n == 0 || d.pixels == 0) return 0;
+  const NormShape s = norm_shape(d);
+  return s.cluster ? 0 : static_cast<size_t>(d.n) * s.spans * d.groups * sizeof(float2);
 }
 
 int8conv_status launch_group_norm_impl(const int8conv_group_norm &d, const void *x, void *y,
                                        void *workspace, cudaStream_t stream) {
+  const NormShape shape = norm_shape(d);
   NormArgs a{};
   a.x = x;
   a.y = y;
@@ -343,14 +672,12 @@ int8conv_status launch_group_norm_impl(const int8conv_group_norm &d, const void 
   a.partial = static_cast<float2 *>(workspace);
   a.ldx = d.ldx;
   a.ldy = d.ldy;
-  a.pixels = d.pixels;
+  a.pixels = static_cast<int32_t>(d.pixels);
   a.channels = d.channels;
   a.groups = d.groups;
   a.per_group = d.channels / d.groups;
-  a.chunk_pixels = pick_chunk_pixels(d);
-  a.chunks = static_cast<int32_t>((d.pixels + a.chunk_pixels - 1) / a.chunk_pixels);
-  a.apply_pixels = a.chunk_pixels;
-  a.apply_chunks = a.chunks;
+  a.spans = shape.spans;
+  a.span_pixels = static_cast<int32_t>(shape.span_pixels);
   a.eps = d.eps;
   a.inv_out_scale = d.y_dtype == INT8CONV_INT8 ? 1.0f / d.out_scale : 1.0f;
   a.activation = d.activation;
@@ -361,32 +688,49 @@ int8conv_status launch_group_norm_impl(const int8conv_group_norm &d, const void 
   const bool vec = d.channels % 8 == 0 && (d.ldx * xs) % 16 == 0 && (d.ldy * ys) % ya == 0 &&
                    (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
                    (reinterpret_cast<uintptr_t>(y) & (ya - 1)) == 0;
-  const void *stats = nullptr, *apply = nullptr;
-  switch (d.x_dtype) {
-    case INT8CONV_BF16:
-      kernels_for<INT8CONV_BF16>(vec, d.y_dtype, &stats, &apply);
-      break;
-    case INT8CONV_FP16:
-      kernels_for<INT8CONV_FP16>(vec, d.y_dtype, &stats, &apply);
-      break;
-    case INT8CONV_FP32:
-      kernels_for<INT8CONV_FP32>(vec, d.y_dtype, &stats, &apply);
-      break;
-    default:
-      kernels_for<INT8CONV_INT32>(vec, d.y_dtype, &stats, &apply);
-  }
+  const NormKernels kernels = d.x_dtype == INT8CONV_BF16   ? kernels_for<INT8CONV_BF16>(vec, d.y_dtype)
+                              : d.x_dtype == INT8CONV_FP16 ? kernels_for<INT8CONV_FP16>(vec, d.y_dtype)
+                              : d.x_dtype == INT8CONV_FP32 ? kernels_for<INT8CONV_FP32>(vec, d.y_dtype)
+                                                           : kernels_for<INT8CONV_INT32>(vec, d.y_dtype);
+  const int width = vec ? 8 : 1;
   LaunchPlan plan;
-  plan.func = stats;
-  plan.grid = dim3(static_cast<unsigned>(a.chunks * d.n));
   plan.block = dim3(kThreads);
-  plan.smem = static_cast<uint32_t>((kThreads * (vec ? 8 : 1) + d.channels) * sizeof(float2));
+  plan.grid = dim3(static_cast<unsigned>(d.n * shape.spans));
+  if (shape.cluster) {
+    // Each thread's share of the span, as far as shared memory reaches.
+    const int cols = d.channels / width;
+    int64_t need = 0;
+    for (int col0 = 0; col0 < cols; col0 += kThreads) {
+      const int w = cols - col0 < kThreads ? cols - col0 : kThreads;
+      const int lanes = kThreads / w;
+      need += (shape.span_pixels + lanes - 1) / lanes;
+    }
+    const uint32_t base = norm_smem(width, xs, d.channels, d.groups, 0).total;
+    // A grid of at most one CTA per SM takes more than half an SM's shared
+    // memory, so that no two of them land on the same one.
+    const bool alone = d.n * shape.spans <= device_info().sm_count;
+    const uint32_t limit = alone ? kMaxSmem : kHalfSmem;
+    const int64_t room =
+        base < limit ? (limit - base) / static_cast<uint32_t>(kThreads * width * xs) : 0;
+    // Whole batches, of the wide vectors only.
+    const int64_t batch = xs == 2 ? 4 : 2;
+    a.keep = vec ? static_cast<int32_t>((need < room ? need : room) / batch * batch) : 0;
+    plan.func = kernels.cluster;
+    plan.smem = norm_smem(width, xs, d.channels, d.groups, a.keep).total;
+    if (alone && plan.smem <= kHalfSmem) plan.smem = kHalfSmem + 1024;
+    plan.cluster = static_cast<uint32_t>(shape.spans);
+    if (!ensure_smem_attr(plan.func, static_cast<int>(plan.smem))) return INT8CONV_CUDA_ERROR;
+    plan_args(plan, a);
+    return launch_plan(plan, stream);
+  }
+  plan.func = kernels.stats;
+  plan.smem = norm_smem(width, xs, d.channels, d.groups, 0).total;
   if (!ensure_smem_attr(plan.func, static_cast<int>(plan.smem))) return INT8CONV_CUDA_ERROR;
   plan_args(plan, a);
-  int8conv_status st = launch_plan(plan, stream);
+  const int8conv_status st = launch_plan(plan, stream);
   if (st != INT8CONV_OK) return st;
-  plan.func = apply;
-  plan.grid = dim3(static_cast<unsigned>(a.apply_chunks * d.n));
-  plan.smem = static_cast<uint32_t>(2 * d.groups * sizeof(float));
+  plan.func = kernels.apply;
+  plan.smem = norm_smem(width, xs, d.channels, d.groups, 0).total;
   if (!ensure_smem_attr(plan.func, static_cast<int>(plan.smem))) return INT8CONV_CUDA_ERROR;
   return launch_plan(plan, stream);
 }

@@ -143,16 +143,20 @@ __device__ __forceinline__ void commit_mma(uint64_t *bar) {
 }
 
 // scale, bias and activation of one 32-column block of a thread's row;
-// `table`: (scale, bias) of the block's columns, two columns per float4.
+// `table`: the block's columns in pairs, (scale, scale, bias, bias).
 template <int ACT>
 __device__ __forceinline__ void finish_block(uint32_t (&v)[32], float rs, const float4 *table) {
+  const uint64_t row = f2_pack(rs, rs);
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     const float4 t = table[j];
-    const float a = fmaf(static_cast<float>(static_cast<int32_t>(v[2 * j])) * t.x, rs, t.y);
-    const float b = fmaf(static_cast<float>(static_cast<int32_t>(v[2 * j + 1])) * t.z, rs, t.w);
-    v[2 * j] = __float_as_uint(activate<ACT>(a));
-    v[2 * j + 1] = __float_as_uint(activate<ACT>(b));
+    const uint64_t x = f2_pack(static_cast<float>(static_cast<int32_t>(v[2 * j])),
+                               static_cast<float>(static_cast<int32_t>(v[2 * j + 1])));
+    float a, b;
+    f2_unpack(f2_fma(f2_mul(x, f2_pack(t.x, t.y)), row, f2_pack(t.z, t.w)), a, b);
+    activate2<ACT>(a, b);
+    v[2 * j] = __float_as_uint(a);
+    v[2 * j + 1] = __float_as_uint(b);
   }
 }
 
@@ -470,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kBlockBytes = 32 * 32 * out_bytes<OUT>();
     constexpr int kBuffers = OUT == INT8CONV_FP32 ? 1 : 2;
     uint8_t *staging = smem + plan.staging_off + (warp - 2) * kStageBytes;
-    float2 *table = reinterpret_cast<float2 *>(smem + plan.table_off + (warp - 2) * kTableBytes);
+    float *table = reinterpret_cast<float *>(smem + plan.table_off + (warp - 2) * kTableBytes);
     // The leader's tempty barriers, 8 bytes apart (a pair signals them remotely).
     const uint32_t tempty_at = PAIR ? mapa_shared(smem_u32(tempty), 0) : smem_u32(tempty);
     T *y = static_cast<T *>(g.y);
@@ -488,12 +492,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int64_t at = static_cast<int64_t>(t.group) * g.N;
         for (int b = 0, c0 = 32 * half; c0 < g.bn; ++b, c0 += 64) {
           const int c = t.n0 + c0 + lane;
-          float2 e = make_float2(0.f, 0.f);
+          float scale = 0.f, bias = 0.f;
           if (c < g.N) {
-            e.x = g.col_scale != nullptr ? __ldg(g.col_scale + at + c) : 1.f;
-            e.y = g.bias != nullptr ? __ldg(g.bias + at + c) : 0.f;
+            scale = g.col_scale != nullptr ? __ldg(g.col_scale + at + c) : 1.f;
+            bias = g.bias != nullptr ? __ldg(g.bias + at + c) : 0.f;
           }
-          table[b * 32 + lane] = e;
+          float *pair = table + (b * 16 + (lane >> 1)) * 4 + (lane & 1);
+          pair[0] = scale;
+          pair[2] = bias;
         }
         __syncwarp();
         table_n0 = t.n0;
@@ -529,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld_32x32b_x32(taddr + c0, v);
           tmem_ld_wait();
           if (c0 + 64 >= g.bn || cols <= 64) release();   // this warp's last read of the tile
-          const float4 *tb = reinterpret_cast<const float4 *>(table + b * 32);
+          const float4 *tb = reinterpret_cast<const float4 *>(table) + b * 16;
           switch (g.activation) {
             case INT8CONV_ACT_RELU:
               finish_block<INT8CONV_ACT_RELU>(v, rs, tb);

@@ -7,6 +7,13 @@
 // from L2).  1 to 16 warps share a row, by its length.  The maximum is taken
 // over the bits of |x|, which order as unsigned integers with infinities and
 // then NaN on top, so one reduction also tells that a row is not finite.
+//
+// An IEEE division is some ten instructions, and with one for each element the
+// kernel was bound by them (16384 x 8192 bf16: 158 us, 2.5 TB/s).  Instead the
+// quotient is a product with the rounded reciprocal, off by at most 3 half
+// steps (3 * 2^-24 * 127 = 2.3e-5): where it lies further than that from the
+// middle between two integers, both round alike; the few vectors with an
+// element nearer than 4e-5 are divided.
 #include <cuda_runtime.h>
 
 #include "epilogue.cuh"
@@ -17,7 +24,7 @@ namespace i8c {
 
 namespace {
 
-constexpr int kHold = 4;          // vectors a thread keeps in registers
+constexpr int kHold = 4;          // vectors a thread keeps in registers, as they lie in memory
 constexpr int kMaxRowWarps = 16;
 
 struct QuantizeArgs {
@@ -29,25 +36,57 @@ struct QuantizeArgs {
   int32_t vec_x, vec_q;
 };
 
-// Eight elements from column k0 on, zeros past the row.
+// Eight elements as they lie in memory.
 template <int DT>
-__device__ __forceinline__ void load8(const typename Elem<DT>::type *row, int64_t k0, int64_t k,
-                                      bool vec, float (&f)[8]) {
+struct Raw8 {
   using T = typename Elem<DT>::type;
-  if (vec && k0 + 8 <= k) {
-    constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  static constexpr int kWords = static_cast<int>(sizeof(T)) / 2;
+  uint4 w[kWords];
+
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int j = 0; j < 8 / kPer; ++j) {
-      const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(row + k0) + j);
-      const T *e = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-      for (int t = 0; t < kPer; ++t) f[j * kPer + t] = Elem<DT>::load(e[t]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = k0 + j < k ? Elem<DT>::load(row[k0 + j]) : 0.f;
+    for (int j = 0; j < kWords; ++j) w[j] = make_uint4(0, 0, 0, 0);
   }
-}
+  // From column k0 on; zeros past the row.
+  __device__ __forceinline__ void load(const T *row, int64_t k0, int64_t k, bool vec) {
+    if (vec && k0 + 8 <= k) {
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) w[j] = __ldg(reinterpret_cast<const uint4 *>(row + k0) + j);
+    } else {
+      clear();
+      // Word by word, with constant indices: the vector stays in registers.
+      uint32_t *u = reinterpret_cast<uint32_t *>(w);
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (k0 + j < k) u[j] = reinterpret_cast<const uint32_t *>(row + k0)[j];
+      } else {
+        const uint16_t *h = reinterpret_cast<const uint16_t *>(row + k0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (k0 + j < k) u[j >> 1] |= static_cast<uint32_t>(h[j]) << (16 * (j & 1));
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int j) const {
+    return Elem<DT>::load(reinterpret_cast<const T *>(w)[j]);
+  }
+  // The larger of `top` and the bits of every |x|; 16-bit types two at a time,
+  // each half on its own.
+  __device__ __forceinline__ uint32_t max_bits(uint32_t top) const {
+    const uint32_t *u = reinterpret_cast<const uint32_t *>(w);
+#pragma unroll
+    for (int j = 0; j < 4 * kWords; ++j)
+      top = sizeof(T) == 4 ? max(top, u[j] & 0x7fffffffu) : __vmaxu2(top, u[j] & 0x7fff7fffu);
+    return top;
+  }
+  // The bits of max_bits() as those of one fp32 value (infinite and NaN stay so).
+  static __device__ __forceinline__ uint32_t to_fp32_bits(uint32_t top) {
+    if constexpr (sizeof(T) == 4) return top;
+    const uint16_t h = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
+    return __float_as_uint(Elem<DT>::load(*reinterpret_cast<const T *>(&h)));
+  }
+};
 
 template <int DT, int WARPS>
 __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS)
@@ -66,37 +105,27 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS)
   const bool valid = r >= 0 && r < a.rows;
   const T *row = static_cast<const T *>(a.x) + (valid ? r : 0) * a.ldx;
   const bool vec = a.vec_x != 0;
-  float held[kHold][8];
+  Raw8<DT> held[kHold];
   uint32_t top = 0;
+#pragma unroll
+  for (int h = 0; h < kHold; ++h) {
+    const int64_t k0 = static_cast<int64_t>(h * kRowThreads + t) * 8;
+    if (valid && k0 < a.k)
+      held[h].load(row, k0, a.k, vec);
+    else
+      held[h].clear();
+  }
+#pragma unroll
+  for (int h = 0; h < kHold; ++h) top = held[h].max_bits(top);
   if (valid) {
-#pragma unroll
-    for (int h = 0; h < kHold; ++h) {
-      const int64_t k0 = static_cast<int64_t>(h * kRowThreads + t) * 8;
-      if (k0 < a.k) {
-        load8<DT>(row, k0, a.k, vec, held[h]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) held[h][j] = 0.f;
-      }
-    }
-#pragma unroll
-    for (int h = 0; h < kHold; ++h)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t b = __float_as_uint(held[h][j]) & 0x7fffffffu;
-        top = b > top ? b : top;
-      }
     for (int64_t k0 = static_cast<int64_t>(kHold * kRowThreads + t) * 8; k0 < a.k;
          k0 += kRowThreads * 8) {
-      float f[8];
-      load8<DT>(row, k0, a.k, vec, f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t b = __float_as_uint(f[j]) & 0x7fffffffu;
-        top = b > top ? b : top;
-      }
+      Raw8<DT> f;
+      f.load(row, k0, a.k, vec);
+      top = f.max_bits(top);
     }
   }
+  top = Raw8<DT>::to_fp32_bits(top);
   top = __reduce_max_sync(0xffffffffu, top);
   if constexpr (WARPS > 1) {
     const int warp = threadIdx.x >> 5;
@@ -112,17 +141,39 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS)
   const bool zero = !valid || !finite || scale == 0.f;
   if (t == 0) a.scale[i] = finite ? scale : __uint_as_float(0x7fffffffu);
   int8_t *q = a.q + i * a.ldq;
-  auto put = [&](int64_t k0, const float (&f)[8]) {
+  // Scales below 2^-100 (their reciprocals leave fp32's range) are divided by.
+  const bool divide = scale < 7.8886090522101181e-31f;
+  const float inv = zero ? 0.f : __frcp_rn(scale);
+  auto put = [&](int64_t k0, const Raw8<DT> &f) {
     uint32_t w[2];
+    float near = 0.f;   // largest distance from an integer
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float v[4];
+      uint32_t b[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        // |x / scale| passes 127 only where the scale is a denormal.
-        v[j] = zero ? 0.f : fminf(fmaxf(__fdiv_rn(f[4 * h + j], scale), -127.f), 127.f);
+        // Adding 1.5 * 2^23 rounds to an integer, half to even, whose low byte
+        // is the sum's.
+        const float p = f.get(4 * h + j) * inv;
+        const float t = p + 12582912.f;
+        near = fmaxf(near, fabsf(p - (t - 12582912.f)));
+        b[j] = __float_as_uint(t);
       }
-      w[h] = pack_int8(v[0], v[1], v[2], v[3]);
+      w[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    }
+    if (zero) {
+      w[0] = w[1] = 0;
+    } else if (divide || near > 0.49996f) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // |x / scale| passes 127 only where the scale is a denormal.
+          v[j] = fminf(fmaxf(__fdiv_rn(f.get(4 * h + j), scale), -127.f), 127.f);
+        }
+        w[h] = pack_int8(v[0], v[1], v[2], v[3]);
+      }
     }
     if (a.vec_q != 0 && k0 + 8 <= a.k) {
       *reinterpret_cast<uint2 *>(q + k0) = make_uint2(w[0], w[1]);
@@ -132,12 +183,6 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS)
         if (k0 + j < a.k) q[k0 + j] = static_cast<int8_t>(w[j >> 2] >> (8 * (j & 3)));
     }
   };
-  if (!valid) {
-#pragma unroll
-    for (int h = 0; h < kHold; ++h)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) held[h][j] = 0.f;
-  }
 #pragma unroll
   for (int h = 0; h < kHold; ++h) {
     const int64_t k0 = static_cast<int64_t>(h * kRowThreads + t) * 8;
@@ -145,8 +190,11 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS)
   }
   for (int64_t k0 = static_cast<int64_t>(kHold * kRowThreads + t) * 8; k0 < a.k;
        k0 += kRowThreads * 8) {
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (valid) load8<DT>(row, k0, a.k, vec, f);
+    Raw8<DT> f;
+    if (valid)
+      f.load(row, k0, a.k, vec);
+    else
+      f.clear();
     put(k0, f);
   }
 }

@@ -300,7 +300,8 @@ def _norm_input(g, n, p, c, dtype, mean=0.5, spread=1.0):
 @pytest.mark.parametrize("n,p,c,groups", [(1, 1, 2, 1), (2, 1, 64, 32), (1, 196, 256, 32),
                                           (3, 77, 320, 32), (2, 50, 30, 5), (5, 9, 7, 7),
                                           (1, 1000, 33, 1), (2, 64, 2560, 32), (1, 3, 8192, 8),
-                                          (70, 20, 48, 3)])
+                                          (70, 20, 48, 3), (1, 40, 4096, 4096),
+                                          (2, 5, 8192, 4096), (150, 30, 72, 9)])
 def test_group_norm(cuda, source, n, p, c, groups):
     g = _gen(12)
     x, scale = _norm_input(g, n, p, c, source)

@@ -119,7 +119,7 @@ def _norm(**change):
 
 @pytest.mark.parametrize("change", [
     dict(n=-1), dict(pixels=-1), dict(channels=0), dict(channels=8193, groups=1, ldx=8193, ldy=8193),
-    dict(groups=0), dict(groups=5), dict(ldx=31), dict(ldy=31), dict(x_dtype=_abi.INT8),
+    dict(channels=4097, groups=4097, ldx=4097, ldy=4097), dict(groups=0), dict(groups=5), dict(ldx=31), dict(ldy=31), dict(x_dtype=_abi.INT8),
     dict(y_dtype=_abi.INT32), dict(eps=-1.0), dict(eps=float("nan")), dict(activation=7),
     dict(y_dtype=_abi.INT8), dict(y_dtype=_abi.INT8, out_scale=float("inf"))])
 def test_group_norm_arguments(change):
