@@ -110,14 +110,15 @@ SIGNATURES = {
     "int8conv_launch_requant": (ctypes.c_int, [ctypes.c_int, _SP, _P, _P, _P,
                                                ctypes.POINTER(CRequant), _P, _P, ctypes.c_size_t,
                                                _P]),
-    "int8conv_launch_matmul": (ctypes.c_int, [ctypes.POINTER(CMatmul), _P, _P, _P, _P]),
-    "int8conv_launch_grouped_matmul": (ctypes.c_int, [ctypes.POINTER(CMatmul), _P, _P,
+    # Descriptors as void pointers: a CMatmul / CGroupNorm by reference, or its packed bytes.
+    "int8conv_launch_matmul": (ctypes.c_int, [_P] * 5),
+    "int8conv_launch_grouped_matmul": (ctypes.c_int, [_P, _P, _P,
                                                       ctypes.c_int64, _P, ctypes.c_int32, _P, _P]),
     "int8conv_launch_quantize_rows": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
                                                      _P, ctypes.c_int64, ctypes.c_int64, _P, _P,
                                                      ctypes.c_int64, _P, _P]),
-    "int8conv_group_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(CGroupNorm)]),
-    "int8conv_launch_group_norm": (ctypes.c_int, [ctypes.POINTER(CGroupNorm), _P, _P, _P,
+    "int8conv_group_norm_workspace_bytes": (ctypes.c_size_t, [_P]),
+    "int8conv_launch_group_norm": (ctypes.c_int, [_P, _P, _P, _P,
                                                   ctypes.c_size_t, _P]),
     "int8conv_device_status": (ctypes.c_int, []),
     "int8conv_set_wait_limit_ns": (None, [ctypes.c_uint64]),

@@ -20,10 +20,42 @@ quantize_rows too.
 """
 from __future__ import annotations
 
-from ctypes import byref
+import struct
 
 from . import _abi
-from .api import _stream
+
+# One short call to the GPU takes a few microseconds, so the checks below are
+# written to cost little next to it: attributes are read once, descriptors are
+# packed in one step, and torch is looked up once.
+_MATMUL = struct.Struct("7q4P2if4x")        # int8conv_matmul
+_NORM = struct.Struct("2q2i2q3Pf3if4x")     # int8conv_group_norm
+_torch = None
+_DTYPES: dict = {}
+_raw_stream = None
+
+
+def _load_torch():
+    global _torch, _raw_stream
+    import torch
+
+    _DTYPES.update({getattr(torch, name): code for name, code in _abi.DTYPES.items()})
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    _torch = torch
+    return torch
+
+
+def _device_index() -> int:
+    return (_torch or _load_torch()).cuda.current_device()
+
+
+def _stream_handle(stream, device: int) -> int:
+    if stream is None:
+        if _raw_stream is not None:
+            return _raw_stream(device)
+        return _torch.cuda.current_stream(device).cuda_stream
+    if isinstance(stream, int):
+        return stream
+    return stream.cuda_stream
 
 
 def _fail(name: str, want: str, t) -> None:
@@ -33,14 +65,7 @@ def _fail(name: str, want: str, t) -> None:
                      f"{tuple(t.stride())} on {t.device}")
 
 
-_DTYPES: dict = {}
-
-
 def _dtype_code(dtype) -> int:
-    if not _DTYPES:
-        import torch
-
-        _DTYPES.update({getattr(torch, name): code for name, code in _abi.DTYPES.items()})
     code = _DTYPES.get(dtype)
     if code is None:
         raise ValueError(f"unsupported type {dtype}")
@@ -54,88 +79,88 @@ def _activation(name: str) -> int:
     return code
 
 
-def _device_index() -> int:
-    import torch
-
-    return torch.cuda.current_device()
-
-
-def _on(name: str, t, device: int) -> None:
+def _misplaced(name: str, t, device: int) -> None:
     if not t.is_cuda:
         raise ValueError(f"{name}: expected a CUDA tensor, got one on {t.device}")
-    if t.device.index != device:
-        raise ValueError(f"{name} on {t.device}, but the current CUDA device is cuda:{device}: "
-                         f"launch under torch.cuda.device({t.device.index}) or move the buffers")
+    raise ValueError(f"{name} on {t.device}, but the current CUDA device is cuda:{device}: "
+                     f"launch under torch.cuda.device({t.device.index}) or move the buffers")
 
 
 def _vector(name: str, t, count: int, device: int, dtype=None) -> int:
-    """Address of an optional contiguous fp32 vector of `count` entries."""
+    """Address of an optional contiguous vector of `count` entries (fp32)."""
     if t is None:
         return 0
-    import torch
-
-    if t.dtype != (dtype or torch.float32) or t.numel() != count or not t.is_contiguous():
-        _fail(name, f"a contiguous {dtype or torch.float32} tensor of {count} elements", t)
-    _on(name, t, device)
+    if dtype is None:
+        dtype = _torch.float32
+    if t.dtype != dtype or t.numel() != count or not t.is_contiguous():
+        _fail(name, f"a contiguous {dtype} tensor of {count} elements", t)
+    if t.get_device() != device:
+        _misplaced(name, t, device)
     return t.data_ptr()
 
 
 def _matrix(name: str, t, device: int):
     """(address, rows, columns, pitch) of a matrix with adjacent columns."""
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+    shape = t.shape
+    if len(shape) != 2:
+        _fail(name, "a matrix", t)
+    rows, cols = shape
+    pitch, unit = t.stride()
+    if unit != 1 and cols > 1:
         _fail(name, "a matrix whose columns are adjacent", t)
-    _on(name, t, device)
-    rows, cols = t.shape
-    # One row has no pitch of its own.
-    pitch = t.stride(0) if rows > 1 else cols
-    if pitch < cols:
+    if t.get_device() != device:
+        _misplaced(name, t, device)
+    if rows <= 1:
+        pitch = cols     # one row has no pitch of its own
+    elif pitch < cols:
         _fail(name, "rows that do not overlap", t)
     return t.data_ptr(), rows, cols, pitch
 
 
 def _int8_matrix(name: str, t, device: int):
-    import torch
-
-    if t.dtype != torch.int8:
+    if t.dtype != _torch.int8:
         _fail(name, "an int8 matrix", t)
     ptr, rows, cols, pitch = _matrix(name, t, device)
-    if rows <= 1:
-        pitch = (cols + 15) // 16 * 16
-    elif pitch % 16:
-        raise ValueError(f"{name}: rows are {pitch} bytes apart, which is not a multiple of 16 "
-                         "(quantize_rows returns rows that are)")
+    if pitch & 15:
+        if rows > 1:
+            raise ValueError(f"{name}: rows are {pitch} bytes apart, which is not a multiple of 16 "
+                             "(quantize_rows returns rows that are)")
+        pitch = (pitch + 15) & -16
     return ptr, rows, cols, pitch
 
 
-def _describe(a, b_shape, y, row_scale, col_scale, bias, activation, residual, out_scale, groups,
-              device):
-    a_ptr, m, k, lda = a
-    n, bk, ldb = b_shape
+def _out_step(code: int, out_scale) -> float:
+    if code == _abi.INT8:
+        if out_scale is None:
+            raise ValueError("an int8 result needs out_scale, what one of its steps is worth")
+        return float(out_scale)
+    if out_scale is not None:
+        raise ValueError("out_scale belongs to an int8 result")
+    return 0.0
+
+
+def _describe(m, k, lda, n, bk, ldb, y, row_scale, col_scale, bias, activation, residual, out_scale,
+              groups, device):
+    """(packed int8conv_matmul, address of y)."""
     if bk != k:
         raise ValueError(f"a has {k} columns, b has {bk}")
     y_ptr, ym, yn, ldy = _matrix("y", y, device)
-    if (ym, yn) != (m, n):
+    if ym != m or yn != n:
         _fail("y", f"a {m} x {n} matrix", y)
-    d = _abi.CMatmul()
-    d.m, d.n, d.k, d.lda, d.ldb, d.ldy = m, n, k, lda, ldb, ldy
-    d.y_dtype = _dtype_code(y.dtype)
-    d.activation = _activation(activation)
-    d.row_scale = _vector("row_scale", row_scale, m, device)
-    d.col_scale = _vector("col_scale", col_scale, n * groups, device)
-    d.bias = _vector("bias", bias, n * groups, device)
+    dtype = y.dtype
+    code = _dtype_code(dtype)
+    res_ptr = ldr = 0
     if residual is not None:
-        if residual.dtype != y.dtype:
-            _fail("residual", f"a {y.dtype} matrix, like y", residual)
-        d.residual, rm, rn, d.ldr = _matrix("residual", residual, device)
-        if (rm, rn) != (m, n):
+        if residual.dtype != dtype:
+            _fail("residual", f"a {dtype} matrix, like y", residual)
+        res_ptr, rm, rn, ldr = _matrix("residual", residual, device)
+        if rm != m or rn != n:
             _fail("residual", f"a {m} x {n} matrix", residual)
-    if d.y_dtype == _abi.INT8:
-        if out_scale is None:
-            raise ValueError("an int8 result needs out_scale, what one of its steps is worth")
-        d.out_scale = float(out_scale)
-    elif out_scale is not None:
-        raise ValueError("out_scale belongs to an int8 result")
-    return d, y_ptr
+    return _MATMUL.pack(m, n, k, lda, ldb, ldy, ldr,
+                        _vector("row_scale", row_scale, m, device),
+                        _vector("col_scale", col_scale, n * groups, device),
+                        _vector("bias", bias, n * groups, device), res_ptr,
+                        _activation(activation), code, _out_step(code, out_scale)), y_ptr
 
 
 def launch_matmul(a, b, y, *, row_scale=None, col_scale=None, bias=None, activation: str = "none",
@@ -148,11 +173,12 @@ def launch_matmul(a, b, y, *, row_scale=None, col_scale=None, bias=None, activat
     (it may be `y`).  The sums are exact, the epilogue is fp32 and rounds once."""
     device = _device_index()
     bp, n, bk, ldb = _int8_matrix("b", b, device)
-    am = _int8_matrix("a", a, device)
-    d, y_ptr = _describe(am, (n, bk, ldb), y, row_scale, col_scale, bias, activation, residual,
-                         out_scale, 1, device)
-    _abi.check(_abi.lib.int8conv_launch_matmul(byref(d), am[0], bp, y_ptr, _stream(stream)),
-               "matmul")
+    ap, m, k, lda = _int8_matrix("a", a, device)
+    d, yp = _describe(m, k, lda, n, bk, ldb, y, row_scale, col_scale, bias, activation, residual,
+                      out_scale, 1, device)
+    status = _abi.lib.int8conv_launch_matmul(d, ap, bp, yp, _stream_handle(stream, device))
+    if status:
+        _abi.check(status, "matmul")
 
 
 def launch_grouped_matmul(a, b, offsets, y, *, row_scale=None, col_scale=None, bias=None,
@@ -163,77 +189,61 @@ def launch_grouped_matmul(a, b, offsets, y, *, row_scale=None, col_scale=None, b
     `a` int8 [m, k] sorted by expert; `b` int8 [experts, n, k]; `offsets` int32
     [experts + 1] on the device, ascending; `col_scale` and `bias` [experts, n].
     Rows of `y` outside [offsets[0], offsets[experts]) are left as they were."""
-    import torch
-
     device = _device_index()
-    if b.dim() != 3 or b.dtype != torch.int8:
+    shape = b.shape
+    if len(shape) != 3 or b.dtype != _torch.int8:
         _fail("b", "an int8 tensor [experts, n, k]", b)
-    groups = b.shape[0]
+    groups, n, bk = shape
     if not 1 <= groups <= 1024:
         raise ValueError(f"b: expected 1 to 1024 experts, got {groups}")
-    bp, n, bk, ldb = _int8_matrix("b", b[0], device)
-    group_stride = b.stride(0) if groups > 1 else 0
-    if groups > 1 and (group_stride % 16 or group_stride < (n - 1) * ldb + bk):
-        _fail("b", "experts that do not overlap, a multiple of 16 bytes apart", b)
-    am = _int8_matrix("a", a, device)
-    d, y_ptr = _describe(am, (n, bk, ldb), y, row_scale, col_scale, bias, activation, None,
-                         out_scale, groups, device)
-    o = _vector("offsets", offsets, groups + 1, device, torch.int32)
-    if not o:
-        raise ValueError("offsets: expected an int32 tensor, got None")
-    _abi.check(_abi.lib.int8conv_launch_grouped_matmul(byref(d), am[0], bp, group_stride, o, groups,
-                                                       y_ptr, _stream(stream)), "grouped_matmul")
+    group_stride, ldb, unit = b.stride()
+    if unit != 1 and bk > 1:
+        _fail("b", "a tensor whose last dimension is adjacent", b)
+    if n <= 1:
+        ldb = (bk + 15) & -16
+    if ldb < bk or ldb & 15 or (groups > 1 and (group_stride & 15
+                                                or group_stride < (n - 1) * ldb + bk)):
+        _fail("b", "rows and experts that do not overlap, multiples of 16 bytes apart", b)
+    if groups == 1:
+        group_stride = 0
+    if b.get_device() != device:
+        _misplaced("b", b, device)
+    ap, m, k, lda = _int8_matrix("a", a, device)
+    d, yp = _describe(m, k, lda, n, bk, ldb, y, row_scale, col_scale, bias, activation, None,
+                      out_scale, groups, device)
+    if offsets is None:
+        _fail("offsets", "an int32 tensor", None)
+    status = _abi.lib.int8conv_launch_grouped_matmul(
+        d, ap, b.data_ptr(), group_stride,
+        _vector("offsets", offsets, groups + 1, device, _torch.int32), groups, yp,
+        _stream_handle(stream, device))
+    if status:
+        _abi.check(status, "grouped_matmul")
 
 
-def _int8_rows(rows: int, cols: int, device):
-    """An uninitialised int8 matrix whose pitch is a multiple of 16."""
-    import torch
-
-    pitch = (cols + 15) // 16 * 16
-    t = torch.empty((rows, pitch), dtype=torch.int8, device=device)
-    return t if pitch == cols else t[:, :cols]
-
-
-class _Allocating:
-    """Allocates on the launch's stream, so that what a call frees on return is
-    reused in that stream's order."""
-
-    def __init__(self, stream):
-        import torch
-
-        self.guard = None
-        if stream is not None:
-            if isinstance(stream, int):
-                stream = torch.cuda.ExternalStream(stream)
-            self.guard = torch.cuda.stream(stream)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
-def _result(m: int, n: int, dtype, device, stream):
-    import torch
-
-    with _Allocating(stream):
-        if dtype == torch.int8:
-            return _int8_rows(m, n, device)
-        return torch.empty((m, n), dtype=dtype, device=device)
+def _empty(shape, dtype, like, stream):
+    """An uninitialised tensor on `like`'s device, allocated on the launch's
+    stream, so that what a call frees on return is reused in that stream's
+    order.  int8 rows get a pitch that is a multiple of 16."""
+    torch = _torch or _load_torch()
+    if stream is not None:
+        if isinstance(stream, int):
+            stream = torch.cuda.ExternalStream(stream)
+        with torch.cuda.stream(stream):
+            return _empty(shape, dtype, like, None)
+    if dtype == torch.int8 and shape[-1] & 15:
+        cols = shape[-1]
+        return like.new_empty((*shape[:-1], (cols + 15) & -16), dtype=dtype)[..., :cols]
+    return like.new_empty(shape, dtype=dtype)
 
 
 def matmul(a, b, *, row_scale=None, col_scale=None, bias=None, activation: str = "none",
            residual=None, dtype=None, out_scale=None, stream=None):
     """launch_matmul into a new result of type `dtype` (default: the residual's
     type, else bfloat16)."""
-    import torch
-
     if dtype is None:
-        dtype = residual.dtype if residual is not None else torch.bfloat16
-    y = _result(a.shape[0], b.shape[0], dtype, a.device, stream)
+        dtype = residual.dtype if residual is not None else (_torch or _load_torch()).bfloat16
+    y = _empty((a.shape[0], b.shape[0]), dtype, a, stream)
     launch_matmul(a, b, y, row_scale=row_scale, col_scale=col_scale, bias=bias,
                   activation=activation, residual=residual, out_scale=out_scale, stream=stream)
     return y
@@ -243,9 +253,9 @@ def grouped_matmul(a, b, offsets, *, row_scale=None, col_scale=None, bias=None,
                    activation: str = "none", dtype=None, out_scale=None, stream=None):
     """launch_grouped_matmul into a new result of type `dtype` (default
     bfloat16); rows that belong to no expert are uninitialised."""
-    import torch
-
-    y = _result(a.shape[0], b.shape[1], dtype or torch.bfloat16, a.device, stream)
+    if len(b.shape) != 3:
+        _fail("b", "an int8 tensor [experts, n, k]", b)
+    y = _empty((a.shape[0], b.shape[1]), dtype or (_torch or _load_torch()).bfloat16, a, stream)
     launch_grouped_matmul(a, b, offsets, y, row_scale=row_scale, col_scale=col_scale, bias=bias,
                           activation=activation, out_scale=out_scale, stream=stream)
     return y
@@ -258,36 +268,35 @@ def launch_quantize_rows(x, q, scale, index=None, *, stream=None) -> None:
     `x` [rows, k] in bfloat16, float16 or float32; `q` int8 [m, k]; `scale`
     float32 [m]; `index` int32 [m] on the device.  A row with an infinity or a
     NaN gets scale NaN and zeros; an index outside [0, rows) scale 0 and zeros."""
-    import torch
-
     device = _device_index()
     x_ptr, rows, k, ldx = _matrix("x", x, device)
     code = _dtype_code(x.dtype)
-    if q.dtype != torch.int8:
+    if q.dtype != _torch.int8:
         _fail("q", "an int8 matrix", q)
     q_ptr, m, qk, ldq = _matrix("q", q, device)
     if qk != k:
         _fail("q", f"{k} columns, like x", q)
-    index_ptr = _vector("index", index, m, device, torch.int32)
     if index is None and rows != m:
         _fail("q", f"{rows} rows, like x", q)
-    scale_ptr = _vector("scale", scale, m, device)
-    _abi.check(_abi.lib.int8conv_launch_quantize_rows(
-        m, k, code, x_ptr, rows, ldx, index_ptr or None, q_ptr, ldq, scale_ptr, _stream(stream)),
-        "quantize_rows")
+    if scale is None:
+        _fail("scale", "a float32 tensor", None)
+    status = _abi.lib.int8conv_launch_quantize_rows(
+        m, k, code, x_ptr, rows, ldx, _vector("index", index, m, device, _torch.int32), q_ptr, ldq,
+        _vector("scale", scale, m, device), _stream_handle(stream, device))
+    if status:
+        _abi.check(status, "quantize_rows")
 
 
 def quantize_rows(x, index=None, *, stream=None):
     """launch_quantize_rows into new buffers: (q, scale).  With `index`, row i of
     the result is x[index[i]]: the gather of an expert dispatch."""
-    import torch
-
-    m = x.shape[0] if index is None else index.numel()
-    if x.dim() != 2:
+    shape = x.shape
+    if len(shape) != 2:
         _fail("x", "a matrix", x)
-    with _Allocating(stream):
-        q = _int8_rows(m, x.shape[1], x.device)
-        scale = torch.empty(m, dtype=torch.float32, device=x.device)
+    m = shape[0] if index is None else index.numel()
+    torch = _torch or _load_torch()
+    q = _empty((m, shape[1]), torch.int8, x, stream)
+    scale = _empty((m,), torch.float32, x, stream)
     launch_quantize_rows(x, q, scale, index, stream=stream)
     return q, scale
 
@@ -295,55 +304,47 @@ def quantize_rows(x, index=None, *, stream=None):
 def _pixels(name: str, t, device: int):
     """(address, images, positions, channels, pitch) of a channels-last tensor
     [n, ..., c] whose positions are evenly spaced."""
-    if t.dim() < 2 or (t.stride(-1) != 1 and t.shape[-1] > 1):
-        _fail(name, "a channels-last tensor [n, ..., c]", t)
-    _on(name, t, device)
     shape, strides = t.shape, t.stride()
-    c, positions, pitch = shape[-1], 1, None
-    for size, stride in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+    if len(shape) < 2 or (strides[-1] != 1 and shape[-1] > 1):
+        _fail(name, "a channels-last tensor [n, ..., c]", t)
+    if t.get_device() != device:
+        _misplaced(name, t, device)
+    n, c = shape[0], shape[-1]
+    positions, pitch = 1, None
+    for i in range(len(shape) - 2, -1, -1):
+        size = shape[i]
         if size > 1:
             if pitch is None:
-                pitch = stride
-            elif stride != pitch * positions and t.numel():
+                pitch = strides[i]
+            elif strides[i] != pitch * positions:
                 _fail(name, "evenly spaced positions", t)
         positions *= size
-    n = shape[0]
-    pitch = c if pitch is None else pitch
-    if pitch < c:
+    if pitch is None:
+        pitch = c
+    elif pitch < c:
         _fail(name, "positions that do not overlap", t)
-    pixels = 1
-    for size in shape[1:-1]:
-        pixels *= size
-    return t.data_ptr(), n, pixels, c, pitch
+    return t.data_ptr(), n, positions // n if n else 0, c, pitch
 
 
 def _norm_desc(x, groups, y, gamma, beta, eps, activation, scale, out_scale, device):
+    """(packed int8conv_group_norm, addresses of x and y)."""
     x_ptr, n, pixels, c, ldx = _pixels("x", x, device)
-    if tuple(y.shape) != tuple(x.shape):
+    if y.shape != x.shape:
         _fail("y", f"a tensor of shape {tuple(x.shape)}", y)
     y_ptr, _, _, _, ldy = _pixels("y", y, device)
-    d = _abi.CGroupNorm()
-    d.n, d.pixels, d.channels, d.groups, d.ldx, d.ldy = n, pixels, c, int(groups), ldx, ldy
-    d.scale = _vector("scale", scale, c, device)
-    d.gamma = _vector("gamma", gamma, c, device)
-    d.beta = _vector("beta", beta, c, device)
-    d.eps = float(eps)
-    d.activation = _activation(activation)
-    d.x_dtype, d.y_dtype = _dtype_code(x.dtype), _dtype_code(y.dtype)
-    if d.y_dtype == _abi.INT8:
-        if out_scale is None:
-            raise ValueError("an int8 result needs out_scale, what one of its steps is worth")
-        d.out_scale = float(out_scale)
-    elif out_scale is not None:
-        raise ValueError("out_scale belongs to an int8 result")
-    return d, x_ptr, y_ptr
+    code = _dtype_code(y.dtype)
+    return _NORM.pack(n, pixels, c, int(groups), ldx, ldy, _vector("scale", scale, c, device),
+                      _vector("gamma", gamma, c, device), _vector("beta", beta, c, device),
+                      float(eps), _activation(activation), _dtype_code(x.dtype), code,
+                      _out_step(code, out_scale)), x_ptr, y_ptr
 
 
 def group_norm_workspace_bytes(x, groups: int, y) -> int:
     """Bytes of scratch that launch_group_norm(x, groups, y, ...) needs."""
+    device = _device_index()
     d, _, _ = _norm_desc(x, groups, y, None, None, 1e-5, "none", None,
-                         1.0 if _dtype_code(y.dtype) == _abi.INT8 else None, _device_index())
-    return int(_abi.lib.int8conv_group_norm_workspace_bytes(byref(d)))
+                         1.0 if y.dtype == _torch.int8 else None, device)
+    return _abi.lib.int8conv_group_norm_workspace_bytes(d)
 
 
 def launch_group_norm(x, groups: int, y, gamma=None, beta=None, *, eps: float = 1e-5,
@@ -363,15 +364,19 @@ def launch_group_norm(x, groups: int, y, gamma=None, beta=None, *, eps: float = 
                                  device)
     ws = 0
     if workspace is not None:
-        if not isinstance(workspace, int):
-            _on("workspace", workspace, device)
+        if isinstance(workspace, int):
+            ws = workspace
+        else:
+            if workspace.get_device() != device:
+                _misplaced("workspace", workspace, device)
             size = workspace.numel() * workspace.element_size()
             if not workspace.is_contiguous() or workspace_bytes > size:
                 _fail("workspace", f"{workspace_bytes} contiguous bytes", workspace)
-            workspace = workspace.data_ptr()
-        ws = workspace
-    _abi.check(_abi.lib.int8conv_launch_group_norm(byref(d), x_ptr, y_ptr, ws, int(workspace_bytes),
-                                                   _stream(stream)), "group_norm")
+            ws = workspace.data_ptr()
+    status = _abi.lib.int8conv_launch_group_norm(d, x_ptr, y_ptr, ws, int(workspace_bytes),
+                                                 _stream_handle(stream, device))
+    if status:
+        _abi.check(status, "group_norm")
 
 
 def group_norm(x, groups: int, gamma=None, beta=None, *, eps: float = 1e-5,
@@ -379,23 +384,17 @@ def group_norm(x, groups: int, gamma=None, beta=None, *, eps: float = 1e-5,
     """launch_group_norm into a new result of type `dtype` (default: x's type, or
     bfloat16 for int32).  An int8 result has its positions a multiple of 16 bytes
     apart, as the convolution and the products read them."""
-    import torch
-
-    if dtype is None:
-        dtype = torch.bfloat16 if x.dtype == torch.int32 else x.dtype
     device = _device_index()
-    with _Allocating(stream):
-        if dtype == torch.int8 and x.dim() >= 2:
-            c = x.shape[-1]
-            y = torch.empty((*x.shape[:-1], (c + 15) // 16 * 16), dtype=dtype,
-                            device=x.device)[..., :c]
-        else:
-            y = torch.empty(x.shape, dtype=dtype, device=x.device)
-        d, x_ptr, y_ptr = _norm_desc(x, groups, y, gamma, beta, eps, activation, scale, out_scale,
-                                     device)
-        nbytes = int(_abi.lib.int8conv_group_norm_workspace_bytes(byref(d)))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    _abi.check(_abi.lib.int8conv_launch_group_norm(byref(d), x_ptr, y_ptr,
-                                                   0 if ws is None else ws.data_ptr(), nbytes,
-                                                   _stream(stream)), "group_norm")
+    if dtype is None:
+        dtype = _torch.bfloat16 if x.dtype == _torch.int32 else x.dtype
+    y = _empty(x.shape, dtype, x, stream)
+    d, x_ptr, y_ptr = _norm_desc(x, groups, y, gamma, beta, eps, activation, scale, out_scale,
+                                 device)
+    nbytes = _abi.lib.int8conv_group_norm_workspace_bytes(d)
+    ws = _empty((nbytes,), _torch.uint8, x, stream) if nbytes else None
+    status = _abi.lib.int8conv_launch_group_norm(d, x_ptr, y_ptr,
+                                                 0 if ws is None else ws.data_ptr(), nbytes,
+                                                 _stream_handle(stream, device))
+    if status:
+        _abi.check(status, "group_norm")
     return y

@@ -144,6 +144,16 @@ def test_group_norm_buffers():
         assert LIB.int8conv_launch_group_norm(ctypes.byref(e), None, None, None, 0, None) == _abi.OK
 
 
+def test_packed_descriptors_are_the_structures():
+    assert operators._MATMUL.size == ctypes.sizeof(_abi.CMatmul)
+    assert operators._NORM.size == ctypes.sizeof(_abi.CGroupNorm)
+    d = _abi.CMatmul.from_buffer_copy(operators._MATMUL.pack(*range(1, 14), 0.5))
+    assert [getattr(d, f) for f, _ in d._fields_] == [*range(1, 14), 0.5]
+    d = _abi.CGroupNorm.from_buffer_copy(
+        operators._NORM.pack(1, 2, 3, 4, 5, 6, 7, 8, 9, 0.25, 10, 11, 12, 0.5))
+    assert [getattr(d, f) for f, _ in d._fields_] == [1, 2, 3, 4, 5, 6, 7, 8, 9, 0.25, 10, 11, 12, 0.5]
+
+
 class _Fake:
     """A CUDA tensor's outside, without a GPU."""
 
@@ -157,9 +167,6 @@ class _Fake:
         self._strides = tuple(strides)
         self.device = torch.device("cuda", index) if cuda else torch.device("cpu")
 
-    def dim(self):
-        return len(self.shape)
-
     def stride(self, i=None):
         return self._strides if i is None else self._strides[i]
 
@@ -169,17 +176,17 @@ class _Fake:
     def is_contiguous(self):
         return True
 
+    def get_device(self):
+        return self.device.index if self.is_cuda else -1
+
     def data_ptr(self):
         return A
-
-    def __getitem__(self, i):
-        return _Fake(self.dtype, self.shape[1:], self._strides[1:], self.device.index)
 
 
 @pytest.fixture
 def device0(monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
-    monkeypatch.setattr(operators, "_stream", lambda s: 0)
+    monkeypatch.setattr(operators, "_stream_handle", lambda stream, device: 0)
 
 
 I8, BF, F32, I32 = torch.int8, torch.bfloat16, torch.float32, torch.int32
