@@ -5,17 +5,23 @@
 //
 // One persistent kernel, 10 warps, one CTA per SM or CTA pairs
 // (tcgen05 cta_group::2, 256-row tiles):
-//   warp 0     TMA producer: A and B tiles of 128 bytes of k, 128-byte swizzle,
-//              into an mbarrier ring.  Rows and columns past the matrices and
-//              bytes past k arrive as zeros, so no size has to divide a tile.
+//   warp 0     TMA producer: A and B tiles of 256 bytes of k (two boxes of 128
+//              bytes, 128-byte swizzle) into an mbarrier ring.  Rows and columns
+//              past the matrices and bytes past k arrive as zeros, so no size
+//              has to divide a tile.
 //   warp 1     MMA issuer: tcgen05.mma kind::i8, int32 accumulators in TMEM,
 //              two buffers, so the epilogue of a tile runs under the next one.
+//   Both run as whole warps with one elected lane issuing, so that addresses
+//   and descriptors are uniform values, and with 8 MMAs between barriers: with
+//   one thread and 4 MMAs the issuer needed 490 cycles for each 128 bytes of k
+//   (a commit alone over 200), whatever the tile, against the 512 that the
+//   largest tile computes.
 //   warps 2-9  epilogue, two warps for each TMEM lane quarter, each taking
-//              every other 32-column block: one row per thread, the column
-//              scales and biases of the tile in shared memory, the residual
-//              read straight into registers, one rounding to the output type,
-//              then a 32 x 32 block staged in swizzled shared memory and written
-//              by one TMA store (or, where the pitch or a ragged group's end
+//              every other 32 columns (64 for int8 output): one row per thread,
+//              the column scales and biases of the tile in shared memory, the
+//              residual read straight into registers, one rounding to the
+//              output type, then 32 x 32 blocks staged in swizzled shared
+//              memory and each written by one TMA store (or, where the pitch or a ragged group's end
 //              does not allow one, by row segments of 16 bytes or elements).
 // A rows are loaded in boxes of 8 to 128 rows (fewer for few tokens): the tile
 // rows that no box covers keep whatever the ring held.  They are integers, so
@@ -40,16 +46,16 @@ namespace i8c {
 
 namespace {
 
-constexpr int kBlockK = 128;                  // bytes of k per stage
+constexpr int kBlockK = 128;                  // bytes of k of one swizzled box
+constexpr int kSub = 2;                       // boxes of each operand in a stage
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
-constexpr int kStageBytes = 4096;             // epilogue staging per warp
 constexpr int kTableBytes = 1024;             // 128 columns x (scale, bias) per warp
-constexpr int kMaxStages = 12;
+constexpr int kMaxStages = 14;
 
 struct MatmulGeom {
   int32_t M, N;
-  int32_t kblocks;
+  int32_t kblocks;     // boxes of 128 bytes of k
   int32_t bn;          // tile width (multiple of 32)
   int32_t a_rows;      // rows of one A box (8..128)
   int32_t n_tiles, m_tiles;
@@ -69,19 +75,33 @@ struct MatmulGeom {
   const int32_t *offsets;
 };
 
-// Shared-memory plan, identical on host and device.
+template <int OUT>
+__host__ __device__ constexpr int out_bytes() {
+  return OUT == INT8CONV_FP32 ? 4 : OUT == INT8CONV_INT8 ? 1 : 2;
+}
+
+// Epilogue staging of one warp: a 32 x 32 block (two for int8).
+__host__ __device__ constexpr int staging_bytes(int out_size) {
+  return out_size == 4 ? 4096 : 2048;
+}
+
+// Shared-memory plan, identical on host and device.  A boxes take the rows that
+// are loaded; an MMA reads 128 rows from a box's start, the surplus being bytes
+// of other boxes (the rings and the staging that follow the last box are longer
+// than 16 KB).
 struct MatmulSmem {
-  uint32_t a_bytes, b_bytes;   // one stage, this CTA's share
+  uint32_t a_box, b_box;       // bytes of one box, this CTA's share
   uint32_t b_off, staging_off, table_off, bar_off, group_off, total;
 };
 
-__host__ __device__ inline MatmulSmem matmul_smem(int b_rows, int stages, int groups) {
+__host__ __device__ inline MatmulSmem matmul_smem(int a_rows, int b_rows, int stages, int groups,
+                                                  int out_size) {
   MatmulSmem p;
-  p.a_bytes = kBlockM * kBlockK;
-  p.b_bytes = b_rows * kBlockK;
-  p.b_off = stages * p.a_bytes;
-  p.staging_off = p.b_off + stages * p.b_bytes;   // b_rows * 128 is a multiple of 1024
-  p.table_off = p.staging_off + kEpiWarps * kStageBytes;
+  p.a_box = a_rows * kBlockK;
+  p.b_box = b_rows * kBlockK;
+  p.b_off = stages * kSub * p.a_box;
+  p.staging_off = p.b_off + stages * kSub * p.b_box;   // boxes are multiples of 1024 bytes
+  p.table_off = p.staging_off + kEpiWarps * staging_bytes(out_size);
   p.bar_off = p.table_off + kEpiWarps * kTableBytes;
   // full/empty[stages], tfull[2], tempty[2], drain, TMEM slot
   p.group_off = p.bar_off + (2 * stages + 5) * 8 + 8;
@@ -134,6 +154,21 @@ __device__ __forceinline__ Tile tile_at(const MatmulGeom &g, int tile_rows, cons
   return t;
 }
 
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// A wait of the whole warp; the vote makes the outcome uniform.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, const WaitCtx &ctx,
+                                          uint32_t bit) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, ctx, bit));
+}
+
 template <bool PAIR>
 __device__ __forceinline__ void commit_mma(uint64_t *bar) {
   if constexpr (PAIR)
@@ -158,11 +193,6 @@ __device__ __forceinline__ void finish_block(uint32_t (&v)[32], float rs, const 
     v[2 * j] = __float_as_uint(a);
     v[2 * j + 1] = __float_as_uint(b);
   }
-}
-
-template <int OUT>
-constexpr int out_bytes() {
-  return OUT == INT8CONV_FP32 ? 4 : OUT == INT8CONV_INT8 ? 1 : 2;
 }
 
 // 16-byte chunk `j` of row `row` in a staged block, under the TMA swizzle whose
@@ -257,9 +287,19 @@ __device__ __forceinline__ void copy_out(const uint4 *stg, typename Elem<OUT>::t
       }
     }
   } else if (lane < cols) {
+    // Element by element, a row segment per instruction; eight rows are read
+    // before the first is written.
     const T *e = reinterpret_cast<const T *>(stg);
-    for (int r = 0; r < rows; ++r)
-      y[r * ldy + lane] = e[chunk_at<OUT>(r, lane / kPer) * kPer + lane % kPer];
+    T *dst = y + lane;
+    for (int r0 = 0; r0 < rows; r0 += 8) {
+      T t[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        t[u] = e[chunk_at<OUT>(r0 + u, lane / kPer) * kPer + lane % kPer];
+#pragma unroll
+      for (int u = 0; u < 8; ++u, dst += ldy)
+        if (r0 + u < rows) *dst = t[u];
+    }
   }
 }
 
@@ -275,7 +315,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   constexpr int kTileRows = PAIR ? 2 * kBlockM : kBlockM;
-  const MatmulSmem plan = matmul_smem(PAIR ? g.bn / 2 : g.bn, g.stages, GROUPED ? g.groups : 0);
+  const MatmulSmem plan = matmul_smem(g.a_rows, PAIR ? g.bn / 2 : g.bn, g.stages,
+                                      GROUPED ? g.groups : 0, out_bytes<OUT>());
   uint8_t *a_ring = smem;
   uint8_t *b_ring = smem + plan.b_off;
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + plan.bar_off);
@@ -287,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int32_t *row_start = reinterpret_cast<int32_t *>(smem + plan.group_off);
   int32_t *tile_start = row_start + g.groups + 1;
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0);   // uniform
   const int lane = threadIdx.x & 31;
   const WaitCtx wctx{ctl.wait_ns, ctl.status};
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
@@ -359,110 +400,128 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if constexpr (PAIR) cluster_sync_all();   // both CTAs' barriers are set up
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   if constexpr (GROUPED) num_tiles = tile_start[g.groups] * g.n_tiles;
 
   if (warp == 0) {
-    if (lane == 0) {
-      // ---------------- TMA producer ----------------
-      if constexpr (!GROUPED) griddep_wait();
-      int stage = 0;
-      uint32_t phase = 0;
-      long armed = 0;
-      const uint32_t tx = static_cast<uint32_t>(g.a_rows * kBlockK) + plan.b_bytes;
-      bool ok = true;
-      for (int u = first; u < num_tiles && ok; u += step) {
-        const Tile t = tile_at<GROUPED>(g, kTileRows, row_start, tile_start, u);
-        const int m0 = t.m0 + static_cast<int>(rank) * kBlockM;
-        const int n0 = t.n0 + static_cast<int>(rank) * (PAIR ? g.bn / 2 : 0);
-        for (int kb = 0; kb < g.kblocks; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1u, wctx, kStatusTimeoutEmpty)) {
-            ok = false;
-            break;
-          }
-          if (!ctl.starve) {
-            // A pair credits both CTAs' bytes to the leader's barrier.
-            if (leader) {
-              mbar_arrive_expect_tx(&full[stage], (PAIR ? 2u : 1u) * tx);
-              ++armed;
-            }
-            void *adst = a_ring + stage * plan.a_bytes;
-            void *bdst = b_ring + stage * plan.b_bytes;
-            if constexpr (PAIR) {
-              const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);
-              tma_load_3d_pair(adst, &tmap_a, bar, kb * kBlockK, m0, 0);
-              tma_load_3d_pair(bdst, &tmap_b, bar, kb * kBlockK, n0, t.group);
-            } else {
-              tma_load_3d(adst, &tmap_a, &full[stage], kb * kBlockK, m0, 0);
-              tma_load_3d(bdst, &tmap_b, &full[stage], kb * kBlockK, n0, t.group);
-            }
-          }
-          if (++stage == g.stages) {
-            stage = 0;
-            phase ^= 1u;
-          }
+    // ---------------- TMA producer ----------------
+    if constexpr (!GROUPED) griddep_wait();
+    int stage = 0;
+    uint32_t phase = 0;
+    int armed = 0;
+    const uint32_t tx = (PAIR ? 2u : 1u) * (plan.a_box + plan.b_box);   // of one box of each
+    bool ok = true;
+    for (int u = first; u < num_tiles && ok; u += step) {
+      const Tile t = tile_at<GROUPED>(g, kTileRows, row_start, tile_start, u);
+      const int m0 = t.m0 + static_cast<int>(rank) * kBlockM;
+      const int n0 = t.n0 + static_cast<int>(rank) * (PAIR ? g.bn / 2 : 0);
+      for (int kb = 0; kb < g.kblocks; kb += kSub) {
+        if (!warp_wait(&empty[stage], phase ^ 1u, wctx, kStatusTimeoutEmpty)) {
+          ok = false;
+          break;
         }
-      }
-      // Copies still in flight land before the CTA exits: wait for the fills
-      // armed last (the leader's barriers count both CTAs' copies).
-      for (long i = 0, n = armed < g.stages ? armed : g.stages; i < n; ++i) {
-        if (--stage < 0) {
-          stage = g.stages - 1;
+        if (!ctl.starve) {
+          const int boxes = g.kblocks - kb < kSub ? g.kblocks - kb : kSub;
+          if (elect_one()) {
+            // A pair credits both CTAs' bytes to the leader's barrier.
+            if (leader) mbar_arrive_expect_tx(&full[stage], boxes * tx);
+            uint8_t *adst = a_ring + stage * (kSub * plan.a_box);
+            uint8_t *bdst = b_ring + stage * (kSub * plan.b_box);
+#pragma unroll
+            for (int i = 0; i < kSub; ++i) {
+              if (i < boxes) {
+                if constexpr (PAIR) {
+                  const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);
+                  tma_load_3d_pair(adst + i * plan.a_box, &tmap_a, bar, (kb + i) * kBlockK, m0, 0);
+                  tma_load_3d_pair(bdst + i * plan.b_box, &tmap_b, bar, (kb + i) * kBlockK, n0,
+                                   t.group);
+                } else {
+                  tma_load_3d(adst + i * plan.a_box, &tmap_a, &full[stage], (kb + i) * kBlockK, m0,
+                              0);
+                  tma_load_3d(bdst + i * plan.b_box, &tmap_b, &full[stage], (kb + i) * kBlockK, n0,
+                              t.group);
+                }
+              }
+            }
+          }
+          __syncwarp();
+          if (leader && armed < g.stages) ++armed;
+        }
+        if (++stage == g.stages) {
+          stage = 0;
           phase ^= 1u;
         }
-        mbar_wait(&full[stage], phase, wctx, kStatusTimeoutTeardown);
       }
     }
+    // Copies still in flight land before the CTA exits: wait for the fills
+    // armed last (the leader's barriers count both CTAs' copies).
+    for (int i = 0; i < armed; ++i) {
+      if (--stage < 0) {
+        stage = g.stages - 1;
+        phase ^= 1u;
+      }
+      warp_wait(&full[stage], phase, wctx, kStatusTimeoutTeardown);
+    }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (leader) {
       // ---------------- MMA issuer (the leader of a pair) ----------------
       const uint32_t idesc = idesc_s8(kTileRows, g.bn);
       const uint64_t a_desc0 = smem_desc(smem_u32(a_ring), 16, 8 * kBlockK, Layout::kSw128);
       const uint64_t b_desc0 = smem_desc(smem_u32(b_ring), 16, 8 * kBlockK, Layout::kSw128);
-      const uint32_t a_step = plan.a_bytes >> 4;
-      const uint32_t b_step = plan.b_bytes >> 4;
+      const uint32_t a_step = plan.a_box >> 4;   // descriptor units, one box on
+      const uint32_t b_step = plan.b_box >> 4;
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       for (int u = first; u < num_tiles && ok; u += step) {
-        if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, wctx, kStatusTimeoutDrain)) break;
+        if (!warp_wait(&tempty[acc], acc_phase ^ 1u, wctx, kStatusTimeoutDrain)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * g.bn);
-        uint32_t accumulate = 0;
-        for (int kb = 0; kb < g.kblocks; ++kb) {
-          if (!mbar_wait(&full[stage], phase, wctx, kStatusTimeoutFull)) {
+        for (int kb = 0; kb < g.kblocks; kb += kSub) {
+          if (!warp_wait(&full[stage], phase, wctx, kStatusTimeoutFull)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint64_t ad = a_desc0 + stage * a_step;
-          const uint64_t bd = b_desc0 + stage * b_step;
+          const int boxes = g.kblocks - kb < kSub ? g.kblocks - kb : kSub;
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < kBlockK / 32; ++k) {
-            if constexpr (PAIR)
-              umma_i8_pair(d_tmem, ad + 2 * k, bd + 2 * k, idesc, accumulate);
-            else
-              umma_i8(d_tmem, ad + 2 * k, bd + 2 * k, idesc, accumulate);
-            accumulate = 1;
+            for (int i = 0; i < kSub; ++i) {
+              if (i < boxes) {
+                const uint64_t ad = a_desc0 + (stage * kSub + i) * a_step;
+                const uint64_t bd = b_desc0 + (stage * kSub + i) * b_step;
+#pragma unroll
+                for (int k = 0; k < kBlockK / 32; ++k) {
+                  const uint32_t accumulate = kb + i + k > 0 ? 1u : 0u;
+                  if constexpr (PAIR)
+                    umma_i8_pair(d_tmem, ad + 2 * k, bd + 2 * k, idesc, accumulate);
+                  else
+                    umma_i8(d_tmem, ad + 2 * k, bd + 2 * k, idesc, accumulate);
+                }
+              }
+            }
+            commit_mma<PAIR>(&empty[stage]);
+            if (kb + kSub >= g.kblocks) commit_mma<PAIR>(&tfull[acc]);
           }
-          commit_mma<PAIR>(&empty[stage]);
+          __syncwarp();
           if (++stage == g.stages) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (!ok) break;
-        commit_mma<PAIR>(&tfull[acc]);
         if (++acc == 2) {
           acc = 0;
           acc_phase ^= 1u;
         }
       }
       // Every MMA issued must finish before TMEM is released (in both CTAs).
-      commit_mma<PAIR>(drain);
-      mbar_wait(drain, 0, wctx, kStatusTimeoutTeardown);
-    } else if (lane == 0 && PAIR) {
-      mbar_wait(drain, 0, wctx, kStatusTimeoutTeardown);
+      // A commit covers the MMAs of the thread that issues it: the lane elected
+      // from the whole warp is always the same one.
+      if (elect_one()) commit_mma<PAIR>(drain);
+      __syncwarp();
+      warp_wait(drain, 0, wctx, kStatusTimeoutTeardown);
+    } else if constexpr (PAIR) {
+      warp_wait(drain, 0, wctx, kStatusTimeoutTeardown);
     }
   } else {
     // ---------------- epilogue (warps 2..9) ----------------
@@ -472,14 +531,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quarter = warp & 3;           // TMEM lane quarter this warp may access
     const int half = (warp - 2) >> 2;       // 32-column blocks half, half + 2, ...
     constexpr int kBlockBytes = 32 * 32 * out_bytes<OUT>();
-    constexpr int kBuffers = OUT == INT8CONV_FP32 ? 1 : 2;
-    uint8_t *staging = smem + plan.staging_off + (warp - 2) * kStageBytes;
+    // Columns a step: the blocks that the staging buffer holds.
+    constexpr int kBlocks = staging_bytes(out_bytes<OUT>()) / kBlockBytes;
+    constexpr int kStep = 32 * kBlocks;
+    uint8_t *staging = smem + plan.staging_off + (warp - 2) * staging_bytes(out_bytes<OUT>());
     float *table = reinterpret_cast<float *>(smem + plan.table_off + (warp - 2) * kTableBytes);
     // The leader's tempty barriers, 8 bytes apart (a pair signals them remotely).
     const uint32_t tempty_at = PAIR ? mapa_shared(smem_u32(tempty), 0) : smem_u32(tempty);
     T *y = static_cast<T *>(g.y);
     const T *residual = static_cast<const T *>(g.residual);
-    int acc = 0, buffer = 0;
+    int acc = 0;
     uint32_t acc_phase = 0;
     int table_n0 = -1, table_group = -1;
     for (int u = first; u < num_tiles; u += step) {
@@ -490,7 +551,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (t.n0 != table_n0 || t.group != table_group) {
         __syncwarp();
         const int64_t at = static_cast<int64_t>(t.group) * g.N;
-        for (int b = 0, c0 = 32 * half; c0 < g.bn; ++b, c0 += 64) {
+        for (int b = 0, c0 = kStep * half; c0 < g.bn;
+             c0 += ++b % kBlocks == 0 ? 32 + kStep : 32) {
           const int c = t.n0 + c0 + lane;
           float scale = 0.f, bias = 0.f;
           if (c < g.N) {
@@ -527,55 +589,68 @@ __global__ void __launch_bounds__(kThreads, 1)
         released = true;
       };
       if (rows > 0) {
-        for (int b = 0, c0 = 32 * half; c0 < g.bn; ++b, c0 += 64) {
+        for (int i = 0, c0 = kStep * half; c0 < g.bn; ++i, c0 += 2 * kStep) {
           const int col0 = t.n0 + c0;
           const int cols = g.N - col0;
           if (cols <= 0) break;
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(taddr + c0, v);
+          // A step is one or two 32-column blocks; the second may lie past the
+          // tile (bn is a multiple of 32 only) or past the matrix.
+          uint32_t v[kBlocks][32];
+#pragma unroll
+          for (int k = 0; k < kBlocks; ++k)
+            if (k == 0 || c0 + 32 < g.bn) tmem_ld_32x32b_x32(taddr + c0 + 32 * k, v[k]);
           tmem_ld_wait();
-          if (c0 + 64 >= g.bn || cols <= 64) release();   // this warp's last read of the tile
-          const float4 *tb = reinterpret_cast<const float4 *>(table) + b * 16;
-          switch (g.activation) {
-            case INT8CONV_ACT_RELU:
-              finish_block<INT8CONV_ACT_RELU>(v, rs, tb);
-              break;
-            case INT8CONV_ACT_GELU:
-              finish_block<INT8CONV_ACT_GELU>(v, rs, tb);
-              break;
-            case INT8CONV_ACT_GELU_TANH:
-              finish_block<INT8CONV_ACT_GELU_TANH>(v, rs, tb);
-              break;
-            case INT8CONV_ACT_SILU:
-              finish_block<INT8CONV_ACT_SILU>(v, rs, tb);
-              break;
-            default:
-              finish_block<INT8CONV_ACT_NONE>(v, rs, tb);
-          }
-          if constexpr (!GROUPED && OUT != INT8CONV_INT8) {
-            if (residual != nullptr && mine)
-              add_residual<OUT>(v, residual + static_cast<int64_t>(row0 + lane) * g.ldr + col0,
-                                cols, g.vec_res != 0);
-          }
-          uint4 *stg = reinterpret_cast<uint4 *>(staging + buffer * kBlockBytes);
-          // The store that last read this buffer has finished reading it.
-          if (lane == 0) bulk_wait_group_read<kBuffers - 1>();
-          __syncwarp();
-          stage_row<OUT>(v, stg, lane, g.inv_out_scale);
+          if (c0 + 2 * kStep >= g.bn || cols <= 2 * kStep) release();   // the tile's last read
+          // The stores that last read the staging buffer have finished reading
+          // it (a step's arithmetic ago).
           const bool tma = g.tma_store != 0 && (!GROUPED || rows >= 32);
+          if (lane == 0) bulk_wait_group_read<0>();
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < kBlocks; ++k) {
+            if (k > 0 && (c0 + 32 >= g.bn || cols <= 32)) break;
+            const float4 *tb = reinterpret_cast<const float4 *>(table) + (i * kBlocks + k) * 16;
+            switch (g.activation) {
+              case INT8CONV_ACT_RELU:
+                finish_block<INT8CONV_ACT_RELU>(v[k], rs, tb);
+                break;
+              case INT8CONV_ACT_GELU:
+                finish_block<INT8CONV_ACT_GELU>(v[k], rs, tb);
+                break;
+              case INT8CONV_ACT_GELU_TANH:
+                finish_block<INT8CONV_ACT_GELU_TANH>(v[k], rs, tb);
+                break;
+              case INT8CONV_ACT_SILU:
+                finish_block<INT8CONV_ACT_SILU>(v[k], rs, tb);
+                break;
+              default:
+                finish_block<INT8CONV_ACT_NONE>(v[k], rs, tb);
+            }
+            if constexpr (!GROUPED && OUT != INT8CONV_INT8) {
+              if (residual != nullptr && mine)
+                add_residual<OUT>(v[k],
+                                  residual + static_cast<int64_t>(row0 + lane) * g.ldr + col0 + 32 * k,
+                                  cols - 32 * k, g.vec_res != 0);
+            }
+            stage_row<OUT>(v[k], reinterpret_cast<uint4 *>(staging + k * kBlockBytes), lane,
+                           g.inv_out_scale);
+          }
           if (tma) fence_proxy_async_smem();
           __syncwarp();
-          if (tma) {
-            if (lane == 0) tma_store_2d(&tmap_y, stg, col0, row0);
-          } else {
-            copy_out<OUT>(stg, y + static_cast<int64_t>(row0) * g.ldy + col0, g.ldy,
-                          rows < 32 ? rows : 32, cols < 32 ? cols : 32, g.vec_store != 0, lane);
+#pragma unroll
+          for (int k = 0; k < kBlocks; ++k) {
+            if (k > 0 && (c0 + 32 >= g.bn || cols <= 32)) break;
+            const uint4 *stg = reinterpret_cast<const uint4 *>(staging + k * kBlockBytes);
+            if (tma) {
+              if (lane == 0) tma_store_2d(&tmap_y, stg, col0 + 32 * k, row0);
+            } else {
+              copy_out<OUT>(stg, y + static_cast<int64_t>(row0) * g.ldy + col0 + 32 * k, g.ldy,
+                            rows < 32 ? rows : 32, cols - 32 * k < 32 ? cols - 32 * k : 32,
+                            g.vec_store != 0, lane);
+            }
           }
-          // One group per block (empty after copy_out), so that the wait above
-          // counts blocks; the block ends together before its buffer's next use.
-          if (lane == 0) bulk_commit_group();
+          if (tma && lane == 0) bulk_commit_group();
           __syncwarp();
-          buffer = buffer + 1 == kBuffers ? 0 : buffer + 1;
         }
       }
       if (!released) release();   // no row or column of this tile for this warp
@@ -616,9 +691,10 @@ struct TileChoice {
 // The candidate with the least estimated time.  Per 128 bytes of k a CTA's
 // tensor core needs 2 * bn cycles (128 x bn x 32 bytes in bn / 2 cycles; a pair
 // 256 x bn in the same), and its loads (a_rows rows of A and its share of B,
-// 128 bytes each) come at about 64 bytes a cycle when all SMs load; the slower
-// of both counts, times the waves of tiles over the SMs, plus a per-tile cost
-// (pipeline fill and the last epilogue).
+// 128 bytes each) come at about 64 bytes a cycle when all SMs load.  The
+// epilogue of the tile before runs meanwhile, some 24 cycles a column.  The
+// slowest of the three counts, times the waves of tiles over the SMs, plus the
+// last epilogue.
 TileChoice choose_tile(int64_t row_tiles128, int64_t row_tiles256, int64_t n, int kblocks,
                        int a_rows, int sms) {
   TileChoice best{false, 128};
@@ -630,19 +706,18 @@ TileChoice choose_tile(int64_t row_tiles128, int64_t row_tiles256, int64_t n, in
     const double waves = static_cast<double>((tiles + slots - 1) / slots);
     const double mma = 2.0 * bn;
     const double load = 2.0 * ((pair ? kBlockM : a_rows) + (pair ? bn / 2 : bn));
-    const double cost = waves * (kblocks * (mma > load ? mma : load) + 4.0 * bn) + 1500.0;
+    const double main = kblocks * (mma > load ? mma : load), finish = 24.0 * bn;
+    const double cost = waves * ((main > finish ? main : finish) + 200.0) + finish;
     if (cost < best_cost * 0.999) {
       best_cost = cost;
       best = TileChoice{pair, bn};
     }
   };
   if (a_rows == kBlockM && pairing_mode() != 1) {
-    consider(true, 256);
-    consider(true, 128);
+    for (int bn = 256; bn >= 64; bn -= 32) consider(true, bn);
     if (pairing_mode() == 2) return best;
   }
-  const int widths[] = {256, 128, 64, 32};
-  for (int bn : widths) consider(false, bn);
+  for (int bn = 256; bn >= 32; bn -= 32) consider(false, bn);
   return best;
 }
 
@@ -747,12 +822,14 @@ int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, co
   if (m_tiles * g.n_tiles >= (int64_t(1) << 30)) return INT8CONV_BAD_ARGUMENT;
   g.m_tiles = static_cast<int32_t>(m_tiles);
   g.band = 8;
-  g.tmem_cols = 2 * g.bn < 32 ? 32 : 2 * g.bn;
+  g.tmem_cols = 32;
+  while (g.tmem_cols < 2 * g.bn) g.tmem_cols *= 2;
   const int b_rows = c.pair ? g.bn / 2 : g.bn;
+  const auto smem_of = [&](int stages) {
+    return matmul_smem(g.a_rows, b_rows, stages, groups, size).total;
+  };
   g.stages = kMaxStages;
-  while (g.stages > 2 &&
-         matmul_smem(b_rows, g.stages, groups).total > static_cast<uint32_t>(kMaxSmem))
-    --g.stages;
+  while (g.stages > 2 && smem_of(g.stages) > static_cast<uint32_t>(kMaxSmem)) --g.stages;
   g.vec_store = (d.ldy * size) % 16 == 0 && aligned(y, 16);
   // A TMA store clips the last column in units of 16 bytes, so a row that ends
   // inside one (in a wider pitch) is stored without it.
@@ -780,7 +857,7 @@ int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, co
   LaunchPlan plan;
   plan.func = c.pair ? (grouped ? kernel_for<true, true>(d.y_dtype) : kernel_for<true, false>(d.y_dtype))
                      : (grouped ? kernel_for<false, true>(d.y_dtype) : kernel_for<false, false>(d.y_dtype));
-  plan.smem = matmul_smem(b_rows, g.stages, groups).total;
+  plan.smem = smem_of(g.stages);
   // At least half an SM's shared memory: one CTA per SM, so that none waits
   // for another's TMEM columns.
   const uint32_t floor_bytes = kMaxSmem / 2 + 1024;
