@@ -17,12 +17,13 @@
 //   (a commit alone over 200), whatever the tile, against the 512 that the
 //   largest tile computes.
 //   warps 2-9  epilogue, two warps for each TMEM lane quarter, each taking
-//              every other 32 columns (64 for int8 output): one row per thread,
-//              the column scales and biases of the tile in shared memory, the
-//              residual read straight into registers, one rounding to the
-//              output type, then 32 x 32 blocks staged in swizzled shared
-//              memory and each written by one TMA store (or, where the pitch or a ragged group's end
-//              does not allow one, by row segments of 16 bytes or elements).
+//              every other 32 columns: one row per thread, the column scales
+//              and biases of the tile in shared memory, the residual read a
+//              block ahead, one rounding to the output type, then blocks of 32
+//              rows x 64 bytes staged in swizzled shared memory and each
+//              written by one TMA store (or, where the pitch or a ragged
+//              group's end does not allow one, by row segments of 16 bytes or
+//              elements).
 // A rows are loaded in boxes of 8 to 128 rows (fewer for few tokens): the tile
 // rows that no box covers keep whatever the ring held.  They are integers, so
 // they can only reach their own accumulator rows, which nothing stores.
@@ -62,7 +63,7 @@ struct MatmulGeom {
   int32_t band;        // row tiles of one band of the tile order
   int32_t stages;
   int32_t tmem_cols;
-  int32_t tma_store;   // 1: whole 32 x 32 blocks leave as TMA stores
+  int32_t tma_store;   // 1: whole blocks leave as TMA stores
   int32_t vec_store;   // 1: rows of y are 16-byte aligned
   int32_t vec_res;     // 1: rows of the residual are 16-byte aligned
   int32_t activation;
@@ -80,10 +81,10 @@ __host__ __device__ constexpr int out_bytes() {
   return OUT == INT8CONV_FP32 ? 4 : OUT == INT8CONV_INT8 ? 1 : 2;
 }
 
-// Epilogue staging of one warp: a 32 x 32 block (two for int8).
-__host__ __device__ constexpr int staging_bytes(int out_size) {
-  return out_size == 4 ? 4096 : 2048;
-}
+// Epilogue staging of one warp: a block of 32 rows x 64 bytes (32 bytes for
+// int8), which is 32 columns, or 16 of fp32.
+constexpr int kStageBytes = 2048;
+__host__ __device__ constexpr int block_cols(int out_size) { return out_size == 4 ? 16 : 32; }
 
 // Shared-memory plan, identical on host and device.  A boxes take the rows that
 // are loaded; an MMA reads 128 rows from a box's start, the surplus being bytes
@@ -94,14 +95,13 @@ struct MatmulSmem {
   uint32_t b_off, staging_off, table_off, bar_off, group_off, total;
 };
 
-__host__ __device__ inline MatmulSmem matmul_smem(int a_rows, int b_rows, int stages, int groups,
-                                                  int out_size) {
+__host__ __device__ inline MatmulSmem matmul_smem(int a_rows, int b_rows, int stages, int groups) {
   MatmulSmem p;
   p.a_box = a_rows * kBlockK;
   p.b_box = b_rows * kBlockK;
   p.b_off = stages * kSub * p.a_box;
   p.staging_off = p.b_off + stages * kSub * p.b_box;   // boxes are multiples of 1024 bytes
-  p.table_off = p.staging_off + kEpiWarps * staging_bytes(out_size);
+  p.table_off = p.staging_off + kEpiWarps * kStageBytes;
   p.bar_off = p.table_off + kEpiWarps * kTableBytes;
   // full/empty[stages], tfull[2], tempty[2], drain, TMEM slot
   p.group_off = p.bar_off + (2 * stages + 5) * 8 + 8;
@@ -196,47 +196,55 @@ __device__ __forceinline__ void finish_block(uint32_t (&v)[32], float rs, const 
 }
 
 // 16-byte chunk `j` of row `row` in a staged block, under the TMA swizzle whose
-// span is the block's row (128, 64 or 32 bytes).
+// span is the block's row (64 or 32 bytes).
 template <int OUT>
 __device__ __forceinline__ int chunk_at(int row, int j) {
-  if constexpr (OUT == INT8CONV_FP32) return row * 8 + (j ^ (row & 7));
   if constexpr (OUT == INT8CONV_INT8) return row * 2 + (j ^ ((row >> 2) & 1));
   return row * 4 + (j ^ ((row >> 1) & 3));
 }
 
-// Adds the residual's 32 columns (row pointer `r`, `cols` of them inside the
-// matrix) to the block.
+// The residual's 32 columns of one row: loaded a block ahead of their use, since
+// a read from memory takes longer than a block's arithmetic (2900 against 800
+// cycles, loaded where they were added).
 template <int OUT>
-__device__ __forceinline__ void add_residual(uint32_t (&v)[32],
-                                             const typename Elem<OUT>::type *r, int cols,
-                                             bool vec) {
+struct ResidualBlock {
   using T = typename Elem<OUT>::type;
-  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
-  if (vec && cols >= 32) {
+  static constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  uint4 w[32 / kPer];
+
+  __device__ __forceinline__ void load(const T *r) {
 #pragma unroll
-    for (int j = 0; j < 32 / kPer; ++j) {
-      const uint4 raw = *reinterpret_cast<const uint4 *>(r + j * kPer);
-      const T *e = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-      for (int t = 0; t < kPer; ++t)
-        v[j * kPer + t] = __float_as_uint(__uint_as_float(v[j * kPer + t]) + Elem<OUT>::load(e[t]));
-    }
-  } else {
+    for (int j = 0; j < 32 / kPer; ++j) w[j] = reinterpret_cast<const uint4 *>(r)[j];
+  }
+  __device__ __forceinline__ void add_to(uint32_t (&v)[32]) const {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (j < cols) v[j] = __float_as_uint(__uint_as_float(v[j]) + Elem<OUT>::load(r[j]));
+      v[j] = __float_as_uint(__uint_as_float(v[j]) +
+                             Elem<OUT>::load(reinterpret_cast<const T *>(w)[j]));
   }
+};
+
+// Element by element: `cols` of the 32 columns at r.
+template <int OUT>
+__device__ __forceinline__ void add_residual(uint32_t (&v)[32],
+                                             const typename Elem<OUT>::type *r, int cols) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (j < cols) v[j] = __float_as_uint(__uint_as_float(v[j]) + Elem<OUT>::load(r[j]));
 }
 
-// One thread's 32 values, rounded, into its row of the staged block.
-template <int OUT>
+// One block's columns of a thread's 32 values, from column FROM on, rounded,
+// into its row of the staged block.
+template <int OUT, int FROM>
 __device__ __forceinline__ void stage_row(const uint32_t (&v)[32], uint4 *stg, int row,
                                           float inv_out_scale) {
   auto f = [&](int i) { return __uint_as_float(v[i]); };
   if constexpr (OUT == INT8CONV_FP32) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      stg[chunk_at<OUT>(row, j)] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    for (int j = 0; j < 4; ++j) {
+      const int i = FROM + 4 * j;
+      stg[chunk_at<OUT>(row, j)] = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    }
   } else if constexpr (OUT == INT8CONV_INT8) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -270,7 +278,7 @@ __device__ __forceinline__ void copy_out(const uint4 *stg, typename Elem<OUT>::t
                                          int rows, int cols, bool vec, int lane) {
   using T = typename Elem<OUT>::type;
   constexpr int kPer = 16 / static_cast<int>(sizeof(T));
-  constexpr int kChunks = 32 / kPer;           // 16-byte chunks per row
+  constexpr int kChunks = block_cols(sizeof(T)) / kPer;   // 16-byte chunks per row
   constexpr int kRows = 32 / kChunks;          // rows per pass of the warp
   if (vec) {
     const int j = lane % kChunks;
@@ -316,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   constexpr int kTileRows = PAIR ? 2 * kBlockM : kBlockM;
   const MatmulSmem plan = matmul_smem(g.a_rows, PAIR ? g.bn / 2 : g.bn, g.stages,
-                                      GROUPED ? g.groups : 0, out_bytes<OUT>());
+                                      GROUPED ? g.groups : 0);
   uint8_t *a_ring = smem;
   uint8_t *b_ring = smem + plan.b_off;
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + plan.bar_off);
@@ -530,11 +538,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 2) griddep_launch_dependents();
     const int quarter = warp & 3;           // TMEM lane quarter this warp may access
     const int half = (warp - 2) >> 2;       // 32-column blocks half, half + 2, ...
-    constexpr int kBlockBytes = 32 * 32 * out_bytes<OUT>();
-    // Columns a step: the blocks that the staging buffer holds.
-    constexpr int kBlocks = staging_bytes(out_bytes<OUT>()) / kBlockBytes;
-    constexpr int kStep = 32 * kBlocks;
-    uint8_t *staging = smem + plan.staging_off + (warp - 2) * staging_bytes(out_bytes<OUT>());
+    constexpr int kCols = block_cols(out_bytes<OUT>());
+    uint8_t *staging = smem + plan.staging_off + (warp - 2) * kStageBytes;
     float *table = reinterpret_cast<float *>(smem + plan.table_off + (warp - 2) * kTableBytes);
     // The leader's tempty barriers, 8 bytes apart (a pair signals them remotely).
     const uint32_t tempty_at = PAIR ? mapa_shared(smem_u32(tempty), 0) : smem_u32(tempty);
@@ -551,8 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (t.n0 != table_n0 || t.group != table_group) {
         __syncwarp();
         const int64_t at = static_cast<int64_t>(t.group) * g.N;
-        for (int b = 0, c0 = kStep * half; c0 < g.bn;
-             c0 += ++b % kBlocks == 0 ? 32 + kStep : 32) {
+        for (int b = 0, c0 = 32 * half; c0 < g.bn; ++b, c0 += 64) {
           const int c = t.n0 + c0 + lane;
           float scale = 0.f, bias = 0.f;
           if (c < g.N) {
@@ -569,6 +573,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       float rs = 1.f;
       if (g.row_scale != nullptr) rs = mine ? __ldg(g.row_scale + row0 + lane) : 0.f;
+      // This row of the residual, and its block that the loop adds next.
+      constexpr bool kResidual = !GROUPED && OUT != INT8CONV_INT8;
+      using Block = ResidualBlock<kResidual ? OUT : INT8CONV_BF16>;
+      Block ahead;
+      const T *res = nullptr;
+      if constexpr (kResidual) {
+        if (residual != nullptr && mine) {
+          res = residual + static_cast<int64_t>(row0 + lane) * g.ldr + t.n0;
+          if (g.vec_res && 32 * half < g.bn && t.n0 + 32 * half + 32 <= g.N)
+            ahead.load(res + 32 * half);
+        }
+      }
       // All lanes wait; the vote keeps the warp converged for tcgen05.ld even
       // if the wait runs out on some lanes only.
       if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_phase, wctx, kStatusTimeoutAccum)))
@@ -589,68 +605,69 @@ __global__ void __launch_bounds__(kThreads, 1)
         released = true;
       };
       if (rows > 0) {
-        for (int i = 0, c0 = kStep * half; c0 < g.bn; ++i, c0 += 2 * kStep) {
+        for (int i = 0, c0 = 32 * half; c0 < g.bn; ++i, c0 += 64) {
           const int col0 = t.n0 + c0;
           const int cols = g.N - col0;
           if (cols <= 0) break;
-          // A step is one or two 32-column blocks; the second may lie past the
-          // tile (bn is a multiple of 32 only) or past the matrix.
-          uint32_t v[kBlocks][32];
-#pragma unroll
-          for (int k = 0; k < kBlocks; ++k)
-            if (k == 0 || c0 + 32 < g.bn) tmem_ld_32x32b_x32(taddr + c0 + 32 * k, v[k]);
+          Block now;
+          if constexpr (kResidual) {
+            now = ahead;
+            if (res != nullptr && g.vec_res && c0 + 64 < g.bn && cols >= 96) ahead.load(res + c0 + 64);
+          }
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(taddr + c0, v);
           tmem_ld_wait();
-          if (c0 + 2 * kStep >= g.bn || cols <= 2 * kStep) release();   // the tile's last read
-          // The stores that last read the staging buffer have finished reading
-          // it (a step's arithmetic ago).
+          if (c0 + 64 >= g.bn || cols <= 64) release();   // this warp's last read of the tile
+          const float4 *tb = reinterpret_cast<const float4 *>(table) + i * 16;
+          switch (g.activation) {
+            case INT8CONV_ACT_RELU:
+              finish_block<INT8CONV_ACT_RELU>(v, rs, tb);
+              break;
+            case INT8CONV_ACT_GELU:
+              finish_block<INT8CONV_ACT_GELU>(v, rs, tb);
+              break;
+            case INT8CONV_ACT_GELU_TANH:
+              finish_block<INT8CONV_ACT_GELU_TANH>(v, rs, tb);
+              break;
+            case INT8CONV_ACT_SILU:
+              finish_block<INT8CONV_ACT_SILU>(v, rs, tb);
+              break;
+            default:
+              finish_block<INT8CONV_ACT_NONE>(v, rs, tb);
+          }
+          if constexpr (kResidual) {
+            if (res != nullptr) {
+              if (g.vec_res && cols >= 32)
+                now.add_to(v);
+              else
+                add_residual<OUT>(v, res + c0, cols);
+            }
+          }
+          uint4 *stg = reinterpret_cast<uint4 *>(staging);
           const bool tma = g.tma_store != 0 && (!GROUPED || rows >= 32);
-          if (lane == 0) bulk_wait_group_read<0>();
-          __syncwarp();
-#pragma unroll
-          for (int k = 0; k < kBlocks; ++k) {
-            if (k > 0 && (c0 + 32 >= g.bn || cols <= 32)) break;
-            const float4 *tb = reinterpret_cast<const float4 *>(table) + (i * kBlocks + k) * 16;
-            switch (g.activation) {
-              case INT8CONV_ACT_RELU:
-                finish_block<INT8CONV_ACT_RELU>(v[k], rs, tb);
-                break;
-              case INT8CONV_ACT_GELU:
-                finish_block<INT8CONV_ACT_GELU>(v[k], rs, tb);
-                break;
-              case INT8CONV_ACT_GELU_TANH:
-                finish_block<INT8CONV_ACT_GELU_TANH>(v[k], rs, tb);
-                break;
-              case INT8CONV_ACT_SILU:
-                finish_block<INT8CONV_ACT_SILU>(v[k], rs, tb);
-                break;
-              default:
-                finish_block<INT8CONV_ACT_NONE>(v[k], rs, tb);
-            }
-            if constexpr (!GROUPED && OUT != INT8CONV_INT8) {
-              if (residual != nullptr && mine)
-                add_residual<OUT>(v[k],
-                                  residual + static_cast<int64_t>(row0 + lane) * g.ldr + col0 + 32 * k,
-                                  cols - 32 * k, g.vec_res != 0);
-            }
-            stage_row<OUT>(v[k], reinterpret_cast<uint4 *>(staging + k * kBlockBytes), lane,
-                           g.inv_out_scale);
-          }
-          if (tma) fence_proxy_async_smem();
-          __syncwarp();
-#pragma unroll
-          for (int k = 0; k < kBlocks; ++k) {
-            if (k > 0 && (c0 + 32 >= g.bn || cols <= 32)) break;
-            const uint4 *stg = reinterpret_cast<const uint4 *>(staging + k * kBlockBytes);
+          auto put = [&](auto from) {
+            constexpr int kFrom = decltype(from)::value;
+            if (kFrom >= cols) return;
+            // The store that last read the buffer has finished reading it.
+            if (lane == 0) bulk_wait_group_read<0>();
+            __syncwarp();
+            stage_row<OUT, kFrom>(v, stg, lane, g.inv_out_scale);
+            if (tma) fence_proxy_async_smem();
+            __syncwarp();
             if (tma) {
-              if (lane == 0) tma_store_2d(&tmap_y, stg, col0 + 32 * k, row0);
+              if (lane == 0) {
+                tma_store_2d(&tmap_y, stg, col0 + kFrom, row0);
+                bulk_commit_group();
+              }
             } else {
-              copy_out<OUT>(stg, y + static_cast<int64_t>(row0) * g.ldy + col0 + 32 * k, g.ldy,
-                            rows < 32 ? rows : 32, cols - 32 * k < 32 ? cols - 32 * k : 32,
-                            g.vec_store != 0, lane);
+              const int wide = cols - kFrom < kCols ? cols - kFrom : kCols;
+              copy_out<OUT>(stg, y + static_cast<int64_t>(row0) * g.ldy + col0 + kFrom, g.ldy,
+                            rows < 32 ? rows : 32, wide, g.vec_store != 0, lane);
             }
-          }
-          if (tma && lane == 0) bulk_commit_group();
-          __syncwarp();
+            __syncwarp();
+          };
+          put(std::integral_constant<int, 0>());
+          if constexpr (kCols == 16) put(std::integral_constant<int, 16>());
         }
       }
       if (!released) release();   // no row or column of this tile for this warp
@@ -688,27 +705,30 @@ struct TileChoice {
   int bn;
 };
 
-// The candidate with the least estimated time.  Per 128 bytes of k a CTA's
-// tensor core needs 2 * bn cycles (128 x bn x 32 bytes in bn / 2 cycles; a pair
-// 256 x bn in the same), and its loads (a_rows rows of A and its share of B,
-// 128 bytes each) come at about 64 bytes a cycle when all SMs load.  The
-// epilogue of the tile before runs meanwhile, some 24 cycles a column.  The
-// slowest of the three counts, times the waves of tiles over the SMs, plus the
-// last epilogue.
-TileChoice choose_tile(int64_t row_tiles128, int64_t row_tiles256, int64_t n, int kblocks,
-                       int a_rows, int sms) {
+// The candidate with the least estimated time, in cycles.  For each 128 bytes
+// of k a CTA's tensor core needs 2 * bn (128 x bn x 32 bytes in bn / 2; a pair
+// 256 x bn in the same), its loads (a_rows rows of A and its share of B, 128
+// bytes each) come at about 80 bytes a cycle, and the issuer needs 285; the
+// slowest counts.  The epilogue of the tile before runs meanwhile.  A pair
+// loses about 2500 cycles between two tiles and 1000 at the start.  The rates
+// were fitted to 20 plain and grouped shapes timed at every width, single and
+// in pairs: the choice is within 3 % of the fastest on each (2048 x 4096 x 4096:
+// pairs of 256 columns 27.7 us, best of 15 27.7, worst 69; 32768 x 320 x 320:
+// single, 160 columns, 11.9 us, worst 21.6).
+TileChoice choose_tile(double row_tiles128, double row_tiles256, int64_t n, int kblocks, int a_rows,
+                       int sms) {
   TileChoice best{false, 128};
   double best_cost = 1e300;
   auto consider = [&](bool pair, int bn) {
-    const int64_t n_tiles = (n + bn - 1) / bn;
-    const int64_t tiles = (pair ? row_tiles256 : row_tiles128) * n_tiles;
-    const int64_t slots = pair ? sms / 2 : sms;
-    const double waves = static_cast<double>((tiles + slots - 1) / slots);
+    const double tiles = (pair ? row_tiles256 : row_tiles128) * static_cast<double>((n + bn - 1) / bn);
+    const double waves = ceil(tiles / (pair ? sms / 2 : sms) - 1e-9);
     const double mma = 2.0 * bn;
-    const double load = 2.0 * ((pair ? kBlockM : a_rows) + (pair ? bn / 2 : bn));
-    const double main = kblocks * (mma > load ? mma : load), finish = 24.0 * bn;
-    const double cost = waves * ((main > finish ? main : finish) + 200.0) + finish;
-    if (cost < best_cost * 0.999) {
+    const double load = (a_rows + (pair ? bn / 2 : bn)) * (kBlockK / 80.0);
+    const double box = fmax(fmax(mma, load), 285.0);
+    const double finish = 5.0 * bn;
+    const double cost = waves * (fmax(kblocks * box, finish) + (pair ? 2500.0 : 100.0)) + finish +
+                        (pair ? 1000.0 : 0.0);
+    if (cost < best_cost) {
       best_cost = cost;
       best = TileChoice{pair, bn};
     }
@@ -750,22 +770,21 @@ bool operand_map(CUtensorMap *map, const int8_t *p, int64_t k, int64_t rows, int
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Output [M][N], boxes of 32 x 32 elements, swizzled over the box's row.
+// Output [M][N], boxes of one staged block, swizzled over the box's row.
 bool result_map(CUtensorMap *map, void *y, int dtype, int64_t m, int64_t n, int64_t ldy) {
   const auto encode = encode_tiled();
   if (encode == nullptr) return false;
   const int size = dtype_bytes(dtype);
   cuuint64_t dims[2] = {(cuuint64_t)n, (cuuint64_t)m};
   cuuint64_t strides[1] = {(cuuint64_t)ldy * size};
-  cuuint32_t box[2] = {32, 32};
+  cuuint32_t box[2] = {(cuuint32_t)block_cols(size), 32};
   cuuint32_t estr[2] = {1, 1};
   // Elements are moved, not computed with: unsigned types of the same size.
   const CUtensorMapDataType type = size == 4   ? CU_TENSOR_MAP_DATA_TYPE_UINT32
                                    : size == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
                                                : CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  const CUtensorMapSwizzle swizzle = size == 4   ? CU_TENSOR_MAP_SWIZZLE_128B
-                                     : size == 2 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                                 : CU_TENSOR_MAP_SWIZZLE_32B;
+  const CUtensorMapSwizzle swizzle =
+      size == 1 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B;
   return encode(map, type, 2, y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                 CU_TENSOR_MAP_L2_PROMOTION_NONE,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -804,15 +823,16 @@ int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, co
   g.a_rows = 8;
   while (g.a_rows < kBlockM && g.a_rows < d.m) g.a_rows *= 2;
   // Row tiles: exact for a plain product; grouped, those of experts that share
-  // the rows evenly (the host does not know the offsets).
-  int64_t tiles128 = (d.m + 127) / 128, tiles256 = (d.m + 255) / 256;
-  if (grouped) {
+  // the rows about evenly (the host does not know the offsets): half a tile of
+  // each is empty.
+  const auto row_tiles = [&](int64_t rows) -> double {
+    if (!grouped) return static_cast<double>((d.m + rows - 1) / rows);
     const int64_t active = groups < d.m ? groups : d.m;
-    const int64_t each = (d.m + active - 1) / active;
-    tiles128 = active * ((each + 127) / 128);
-    tiles256 = active * ((each + 255) / 256);
-  }
-  const TileChoice c = choose_tile(tiles128, tiles256, d.n, g.kblocks, g.a_rows, sms);
+    const double each = static_cast<double>(d.m) / active;
+    return active * fmax(1.0, each / rows + 0.5);
+  };
+  const TileChoice c = choose_tile(row_tiles(kBlockM), row_tiles(2 * kBlockM), d.n, g.kblocks,
+                                   g.a_rows, sms);
   g.bn = c.bn;
   const int tile_rows = c.pair ? 2 * kBlockM : kBlockM;
   g.n_tiles = static_cast<int32_t>((d.n + g.bn - 1) / g.bn);
@@ -826,7 +846,7 @@ int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, co
   while (g.tmem_cols < 2 * g.bn) g.tmem_cols *= 2;
   const int b_rows = c.pair ? g.bn / 2 : g.bn;
   const auto smem_of = [&](int stages) {
-    return matmul_smem(g.a_rows, b_rows, stages, groups, size).total;
+    return matmul_smem(g.a_rows, b_rows, stages, groups).total;
   };
   g.stages = kMaxStages;
   while (g.stages > 2 && smem_of(g.stages) > static_cast<uint32_t>(kMaxSmem)) --g.stages;
