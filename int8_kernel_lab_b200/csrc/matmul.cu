@@ -24,9 +24,10 @@
 //              written by one TMA store (or, where the pitch or a ragged
 //              group's end does not allow one, by row segments of 16 bytes or
 //              elements).
-// A rows are loaded in boxes of 8 to 128 rows (fewer for few tokens): the tile
-// rows that no box covers keep whatever the ring held.  They are integers, so
-// they can only reach their own accumulator rows, which nothing stores.
+// A rows are loaded in boxes of 8 to 128 rows (smaller for few tokens, and for
+// experts with few rows): the tile rows that no box covers keep whatever the
+// ring held.  They are integers, so they can only reach their own accumulator
+// rows, which nothing stores.
 //
 // Grouped: A rows are sorted by expert and B is [groups][n][k].  Every CTA
 // scans the device-side offsets into a table of row tiles in shared memory, and
@@ -58,7 +59,8 @@ struct MatmulGeom {
   int32_t M, N;
   int32_t kblocks;     // boxes of 128 bytes of k
   int32_t bn;          // tile width (multiple of 32)
-  int32_t a_rows;      // rows of one A box (8..128)
+  int32_t a_rows;      // rows of A that a stage has room for (8..128)
+  int32_t box_rows;    // rows of one A box: a tile loads as many as its rows need
   int32_t n_tiles, m_tiles;
   int32_t band;        // row tiles of one band of the tile order
   int32_t stages;
@@ -417,12 +419,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     int stage = 0;
     uint32_t phase = 0;
     int armed = 0;
-    const uint32_t tx = (PAIR ? 2u : 1u) * (plan.a_box + plan.b_box);   // of one box of each
+    const uint32_t box_bytes = static_cast<uint32_t>(g.box_rows * kBlockK);
     bool ok = true;
     for (int u = first; u < num_tiles && ok; u += step) {
       const Tile t = tile_at<GROUPED>(g, kTileRows, row_start, tile_start, u);
       const int m0 = t.m0 + static_cast<int>(rank) * kBlockM;
       const int n0 = t.n0 + static_cast<int>(rank) * (PAIR ? g.bn / 2 : 0);
+      // A plain product's boxes cover the tile; a group's as many as its rows need.
+      int parts = 1;
+      if (GROUPED && !PAIR && g.box_rows < g.a_rows) {
+        const int rows = t.m_end - m0 < g.a_rows ? t.m_end - m0 : g.a_rows;
+        parts = __shfl_sync(0xffffffffu, (rows + g.box_rows - 1) / g.box_rows, 0);
+      }
+      const uint32_t tx = (PAIR ? 2u : 1u) * (parts * box_bytes + plan.b_box);   // 128 bytes of k
       for (int kb = 0; kb < g.kblocks; kb += kSub) {
         if (!warp_wait(&empty[stage], phase ^ 1u, wctx, kStatusTimeoutEmpty)) {
           ok = false;
@@ -444,8 +453,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                   tma_load_3d_pair(bdst + i * plan.b_box, &tmap_b, bar, (kb + i) * kBlockK, n0,
                                    t.group);
                 } else {
-                  tma_load_3d(adst + i * plan.a_box, &tmap_a, &full[stage], (kb + i) * kBlockK, m0,
-                              0);
+                  for (int j = 0; j < parts; ++j)
+                    tma_load_3d(adst + i * plan.a_box + j * box_bytes, &tmap_a, &full[stage],
+                                (kb + i) * kBlockK, m0 + j * g.box_rows, 0);
                   tma_load_3d(bdst + i * plan.b_box, &tmap_b, &full[stage], (kb + i) * kBlockK, n0,
                               t.group);
                 }
@@ -831,8 +841,14 @@ int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, co
     const double each = static_cast<double>(d.m) / active;
     return active * fmax(1.0, each / rows + 0.5);
   };
+  // Experts with few rows each: boxes of about that many rows.
+  g.box_rows = g.a_rows;
+  if (grouped) {
+    const int64_t each = (d.m + groups - 1) / groups;
+    while (g.box_rows > 8 && g.box_rows > each) g.box_rows /= 2;
+  }
   const TileChoice c = choose_tile(row_tiles(kBlockM), row_tiles(2 * kBlockM), d.n, g.kblocks,
-                                   g.a_rows, sms);
+                                   g.box_rows, sms);
   g.bn = c.bn;
   const int tile_rows = c.pair ? 2 * kBlockM : kBlockM;
   g.n_tiles = static_cast<int32_t>((d.n + g.bn - 1) / g.bn);
@@ -868,7 +884,7 @@ int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, co
   g.offsets = offsets;
 
   CUtensorMap tmap_a, tmap_b, tmap_y{};
-  if (!operand_map(&tmap_a, a, d.k, d.m, d.lda, 1, d.lda, g.a_rows) ||
+  if (!operand_map(&tmap_a, a, d.k, d.m, d.lda, 1, d.lda, g.box_rows) ||
       !operand_map(&tmap_b, b, d.k, d.n, d.ldb, grouped ? groups : 1,
                    groups > 1 ? group_stride : d.ldb, b_rows))
     return INT8CONV_CUDA_ERROR;
