@@ -24,19 +24,40 @@ import struct
 
 from . import _abi
 
-# One short call to the GPU takes a few microseconds, so the checks below are
-# written to cost little next to it: attributes are read once, descriptors are
-# packed in one step, and torch is looked up once.
+# One short call to the GPU takes a few microseconds.  The calls that allocate
+# their result and run on the current stream therefore go through torch_calls
+# (csrc/torch_calls.cpp, where it was built), which checks and launches a
+# well-formed call in about one microsecond beside the launch itself and
+# declines every other; what it declines, and every other call, takes the
+# checks below, which name what is wrong.  They too are written to cost little:
+# attributes are read once, descriptors are packed in one step, and torch is
+# looked up once.
 _MATMUL = struct.Struct("7q4P2if4x")        # int8conv_matmul
 _NORM = struct.Struct("2q2i2q3Pf3if4x")     # int8conv_group_norm
+_CALLS_PATH = _abi.LIB_PATH.parent / "torch_calls.so"
 _torch = None
 _DTYPES: dict = {}
 _raw_stream = None
+_calls = None
+
+
+def _load_calls():
+    """The compiled calls, or None where they were not built."""
+    if not _CALLS_PATH.exists():
+        return None
+    import importlib.util
+
+    spec = importlib.util.spec_from_file_location("torch_calls", _CALLS_PATH)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
 
 
 def _load_torch():
-    global _torch, _raw_stream
+    global _torch, _raw_stream, _calls
     import torch
+
+    _calls = _load_calls()
 
     _DTYPES.update({getattr(torch, name): code for name, code in _abi.DTYPES.items()})
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -172,6 +193,10 @@ def launch_matmul(a, b, y, *, row_scale=None, col_scale=None, bias=None, activat
     `col_scale` [n] and `bias` [n] float32, each optional; `residual` like `y`
     (it may be `y`).  The sums are exact, the epilogue is fp32 and rounds once."""
     device = _device_index()
+    if stream is None and _calls is not None and y is not None and _calls.matmul(
+            a, b, None, y, row_scale, col_scale, bias, residual, _activation(activation), 0,
+            out_scale) is not None:
+        return
     bp, n, bk, ldb = _int8_matrix("b", b, device)
     ap, m, k, lda = _int8_matrix("a", a, device)
     d, yp = _describe(m, k, lda, n, bk, ldb, y, row_scale, col_scale, bias, activation, residual,
@@ -190,6 +215,12 @@ def launch_grouped_matmul(a, b, offsets, y, *, row_scale=None, col_scale=None, b
     [experts + 1] on the device, ascending; `col_scale` and `bias` [experts, n].
     Rows of `y` outside [offsets[0], offsets[experts]) are left as they were."""
     device = _device_index()
+    if offsets is None:
+        _fail("offsets", "an int32 tensor", None)
+    if stream is None and _calls is not None and y is not None and _calls.matmul(
+            a, b, offsets, y, row_scale, col_scale, bias, None, _activation(activation), 0,
+            out_scale) is not None:
+        return
     shape = b.shape
     if len(shape) != 3 or b.dtype != _torch.int8:
         _fail("b", "an int8 tensor [experts, n, k]", b)
@@ -211,8 +242,6 @@ def launch_grouped_matmul(a, b, offsets, y, *, row_scale=None, col_scale=None, b
     ap, m, k, lda = _int8_matrix("a", a, device)
     d, yp = _describe(m, k, lda, n, bk, ldb, y, row_scale, col_scale, bias, activation, None,
                       out_scale, groups, device)
-    if offsets is None:
-        _fail("offsets", "an int32 tensor", None)
     status = _abi.lib.int8conv_launch_grouped_matmul(
         d, ap, b.data_ptr(), group_stride,
         _vector("offsets", offsets, groups + 1, device, _torch.int32), groups, yp,
@@ -241,8 +270,14 @@ def matmul(a, b, *, row_scale=None, col_scale=None, bias=None, activation: str =
            residual=None, dtype=None, out_scale=None, stream=None):
     """launch_matmul into a new result of type `dtype` (default: the residual's
     type, else bfloat16)."""
+    torch = _torch or _load_torch()
     if dtype is None:
-        dtype = residual.dtype if residual is not None else (_torch or _load_torch()).bfloat16
+        dtype = residual.dtype if residual is not None else torch.bfloat16
+    if stream is None and _calls is not None:
+        y = _calls.matmul(a, b, None, None, row_scale, col_scale, bias, residual,
+                          _activation(activation), _dtype_code(dtype), out_scale)
+        if y is not None:
+            return y
     y = _empty((a.shape[0], b.shape[0]), dtype, a, stream)
     launch_matmul(a, b, y, row_scale=row_scale, col_scale=col_scale, bias=bias,
                   activation=activation, residual=residual, out_scale=out_scale, stream=stream)
@@ -253,9 +288,19 @@ def grouped_matmul(a, b, offsets, *, row_scale=None, col_scale=None, bias=None,
                    activation: str = "none", dtype=None, out_scale=None, stream=None):
     """launch_grouped_matmul into a new result of type `dtype` (default
     bfloat16); rows that belong to no expert are uninitialised."""
+    torch = _torch or _load_torch()
+    if dtype is None:
+        dtype = torch.bfloat16
+    if offsets is None:
+        _fail("offsets", "an int32 tensor", None)
+    if stream is None and _calls is not None:
+        y = _calls.matmul(a, b, offsets, None, row_scale, col_scale, bias, None,
+                          _activation(activation), _dtype_code(dtype), out_scale)
+        if y is not None:
+            return y
     if len(b.shape) != 3:
         _fail("b", "an int8 tensor [experts, n, k]", b)
-    y = _empty((a.shape[0], b.shape[1]), dtype or (_torch or _load_torch()).bfloat16, a, stream)
+    y = _empty((a.shape[0], b.shape[1]), dtype, a, stream)
     launch_grouped_matmul(a, b, offsets, y, row_scale=row_scale, col_scale=col_scale, bias=bias,
                           activation=activation, out_scale=out_scale, stream=stream)
     return y
@@ -269,6 +314,9 @@ def launch_quantize_rows(x, q, scale, index=None, *, stream=None) -> None:
     float32 [m]; `index` int32 [m] on the device.  A row with an infinity or a
     NaN gets scale NaN and zeros; an index outside [0, rows) scale 0 and zeros."""
     device = _device_index()
+    if stream is None and _calls is not None and q is not None and _calls.quantize_rows(
+            x, index, q, scale) is not None:
+        return
     x_ptr, rows, k, ldx = _matrix("x", x, device)
     code = _dtype_code(x.dtype)
     if q.dtype != _torch.int8:
@@ -290,11 +338,15 @@ def launch_quantize_rows(x, q, scale, index=None, *, stream=None) -> None:
 def quantize_rows(x, index=None, *, stream=None):
     """launch_quantize_rows into new buffers: (q, scale).  With `index`, row i of
     the result is x[index[i]]: the gather of an expert dispatch."""
+    torch = _torch or _load_torch()
+    if stream is None and _calls is not None:
+        pair = _calls.quantize_rows(x, index, None, None)
+        if pair is not None:
+            return pair
     shape = x.shape
     if len(shape) != 2:
         _fail("x", "a matrix", x)
     m = shape[0] if index is None else index.numel()
-    torch = _torch or _load_torch()
     q = _empty((m, shape[1]), torch.int8, x, stream)
     scale = _empty((m,), torch.float32, x, stream)
     launch_quantize_rows(x, q, scale, index, stream=stream)
@@ -387,6 +439,11 @@ def group_norm(x, groups: int, gamma=None, beta=None, *, eps: float = 1e-5,
     device = _device_index()
     if dtype is None:
         dtype = _torch.bfloat16 if x.dtype == _torch.int32 else x.dtype
+    if stream is None and _calls is not None:
+        y = _calls.group_norm(x, groups, gamma, beta, scale, eps, _activation(activation),
+                              _dtype_code(dtype), out_scale)
+        if y is not None:
+            return y
     y = _empty(x.shape, dtype, x, stream)
     d, x_ptr, y_ptr = _norm_desc(x, groups, y, gamma, beta, eps, activation, scale, out_scale,
                                  device)

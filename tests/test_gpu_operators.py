@@ -6,7 +6,7 @@ import torch
 
 import int8_kernel_lab_b200 as m
 import operators_reference as ref
-from int8_kernel_lab_b200 import _abi
+from int8_kernel_lab_b200 import _abi, operators
 
 pytestmark = pytest.mark.gpu
 
@@ -492,6 +492,39 @@ def test_grouped_matmul_captured_reads_new_offsets(cuda):
         graph.replay()
         torch.cuda.synchronize()
         _check_grouped(o, y, before, list(zip(ends, ends[1:])), torch.float32)
+
+
+def test_compiled_and_checked_calls_agree(cuda, monkeypatch):
+    # The calls through torch_calls and those through the Python checks launch
+    # the same kernels on the same arguments, strided and odd ones too.
+    def results():
+        out = []
+        o = _operands(33, 50, 70, 30, extra=16)
+        y, _ = _framed(33, 50, torch.float16, 3, 1)
+        m.launch_matmul(o["a"], o["b"], y, row_scale=o["row"], col_scale=o["col"])
+        out += [y, m.matmul(o["a"][:1], o["b"], bias=o["bias"], activation="gelu"),
+                m.matmul(o["a"], o["b"], col_scale=o["col"], dtype=torch.int8, out_scale=0.5),
+                m.matmul(o["a"], o["b"], residual=o["residual"][:, :50], dtype=torch.float32)]
+        e = _grouped_case([9, 0, 5], 40, 50, 31)
+        out += [m.grouped_matmul(e["a"], e["b"], e["offsets"], row_scale=e["row"],
+                                 col_scale=e["col"], bias=e["bias"], activation="relu")]
+        x = torch.randn(20, 45, generator=_gen(32), device="cuda")
+        index = torch.tensor([4, 4, 19, 0], dtype=torch.int32, device="cuda")
+        q, scale = torch.zeros(20, 45, dtype=torch.int8, device="cuda"), torch.zeros(20, device="cuda")
+        m.launch_quantize_rows(x[:, ::1], q, scale)
+        out += [q, scale, *m.quantize_rows(x, index), *m.quantize_rows(x[:, 3:17])]
+        z = torch.randn(2, 6, 7, 24, generator=_gen(33), device="cuda").to(torch.bfloat16)
+        out += [m.group_norm(z, 4, activation="silu"), m.group_norm(z[..., 8:], 2, dtype=torch.float32),
+                m.group_norm(z, 3, dtype=torch.int8, out_scale=0.1)]
+        return out
+
+    assert operators._calls is not None, "torch_calls.so was not built"
+    fast = results()
+    monkeypatch.setattr(operators, "_calls", None)
+    slow = results()
+    for a, b in zip(fast, slow):
+        assert a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride()
+        assert torch.equal(a, b)
 
 
 def test_timed_out_waits_are_reported(cuda):

@@ -154,6 +154,19 @@ def test_packed_descriptors_are_the_structures():
     assert [getattr(d, f) for f, _ in d._fields_] == [1, 2, 3, 4, 5, 6, 7, 8, 9, 0.25, 10, 11, 12, 0.5]
 
 
+def test_compiled_calls_decline_what_is_not_a_cuda_tensor():
+    operators._load_torch()
+    if operators._calls is None:
+        pytest.skip("torch_calls.so was not built")
+    t = torch.zeros(4, 32, dtype=torch.int8)
+    none = [None] * 6
+    for a in (t, 3, None, "a"):
+        assert operators._calls.matmul(a, t, *none, 0, 0, None) is None
+        assert operators._calls.quantize_rows(a, None, None, None) is None
+        assert operators._calls.group_norm(a, 4, None, None, None, 1e-5, 0, 0, None) is None
+    assert operators._calls.matmul() is None and operators._calls.group_norm(t) is None
+
+
 class _Fake:
     """A CUDA tensor's outside, without a GPU."""
 
