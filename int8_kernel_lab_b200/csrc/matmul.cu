@@ -41,6 +41,7 @@
 
 #include "conv_common.h"
 #include "epilogue.cuh"
+#include "int8conv_rules.h"
 #include "launch.h"
 #include "sm100.cuh"
 
@@ -70,6 +71,7 @@ struct MatmulGeom {
   int32_t vec_res;     // 1: rows of the residual are 16-byte aligned
   int32_t activation;
   int32_t groups;      // 0: plain product
+  int32_t splits;      // CTAs that share a tile's k (split kernel)
   float inv_out_scale;
   int64_t ldy, ldr;    // elements
   const float *row_scale, *col_scale, *bias;
@@ -705,6 +707,240 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+__device__ __forceinline__ int4 ld_cluster_v4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ float activate_any(float v, int activation) {
+  switch (activation) {
+    case INT8CONV_ACT_RELU:
+      return activate<INT8CONV_ACT_RELU>(v);
+    case INT8CONV_ACT_GELU:
+      return activate<INT8CONV_ACT_GELU>(v);
+    case INT8CONV_ACT_GELU_TANH:
+      return activate<INT8CONV_ACT_GELU_TANH>(v);
+    case INT8CONV_ACT_SILU:
+      return activate<INT8CONV_ACT_SILU>(v);
+    default:
+      return v;
+  }
+}
+
+// Few rows: one tile per cluster of g.splits CTAs, each taking a share of k.
+//
+// With few tiles a narrow one on every SM was bound by the tensor core, which
+// reads 128 rows of A for each instruction however few columns it multiplies
+// (16 x 4096 x 4096 in 128 tiles of 32 columns: 128 instructions of 60 cycles a
+// CTA).  Shares of k keep the tiles wide: the same bytes of B for each SM, a
+// quarter of the instructions.  The int32 partial sums of the tile's rows meet
+// in distributed shared memory (the operand ring's, which is free by then); CTA
+// r adds, finishes and stores the r-th share of the columns, four columns a thread.
+// Integer sums are exact, so the split changes no result.
+template <int OUT>
+__global__ void __launch_bounds__(kThreads, 1)
+    matmul_split_kernel(const __grid_constant__ CUtensorMap tmap_a,
+                        const __grid_constant__ CUtensorMap tmap_b, const MatmulGeom g,
+                        const RunCtl ctl) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const MatmulSmem plan = matmul_smem(g.a_rows, g.bn, g.stages, 0);
+  uint8_t *a_ring = smem;
+  uint8_t *b_ring = smem + plan.b_off;
+  int32_t *partial = reinterpret_cast<int32_t *>(smem);
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + plan.bar_off);
+  uint64_t *empty = full + g.stages;
+  uint64_t *tfull = empty + g.stages;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tfull + 5);
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0);   // uniform
+  const int lane = threadIdx.x & 31;
+  const WaitCtx wctx{ctl.wait_ns, ctl.status};
+  const int rank = static_cast<int>(blockIdx.x) % g.splits;
+  const int tile = static_cast<int>(blockIdx.x) / g.splits;
+  const int n0 = tile % g.n_tiles * g.bn;
+  const int m0 = tile / g.n_tiles * kBlockM;
+  const int rows = g.M - m0 < kBlockM ? g.M - m0 : kBlockM;
+  // Shares of k in whole stages; the last ones may be shorter, or empty.
+  const int share = (g.kblocks + g.splits * kSub - 1) / (g.splits * kSub) * kSub;
+  const int kb_begin = rank * share < g.kblocks ? rank * share : g.kblocks;
+  const int kb_end = kb_begin + share < g.kblocks ? kb_begin + share : g.kblocks;
+  const int pitch = g.bn + 4;   // words; 16-byte stores of neighbouring rows meet no bank twice
+
+  if (warp == 0) {
+    for (int i = lane; i < 2 * g.stages + 1; i += 32) mbar_init(&full[i], 1);
+    fence_mbar_init();
+    if (lane == 0) {
+      tma_prefetch_desc(&tmap_a);
+      tma_prefetch_desc(&tmap_b);
+    }
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, g.tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    griddep_wait();
+    int stage = 0, armed = 0;
+    uint32_t phase = 0;
+    for (int kb = kb_begin; kb < kb_end; kb += kSub) {
+      if (!warp_wait(&empty[stage], phase ^ 1u, wctx, kStatusTimeoutEmpty)) break;
+      if (!ctl.starve) {
+        const int boxes = kb_end - kb < kSub ? kb_end - kb : kSub;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&full[stage], boxes * (plan.a_box + plan.b_box));
+          uint8_t *adst = a_ring + stage * (kSub * plan.a_box);
+          uint8_t *bdst = b_ring + stage * (kSub * plan.b_box);
+#pragma unroll
+          for (int i = 0; i < kSub; ++i) {
+            if (i < boxes) {
+              tma_load_3d(bdst + i * plan.b_box, &tmap_b, &full[stage], (kb + i) * kBlockK, n0, 0);
+              tma_load_3d(adst + i * plan.a_box, &tmap_a, &full[stage], (kb + i) * kBlockK, m0, 0);
+            }
+          }
+        }
+        __syncwarp();
+        if (armed < g.stages) ++armed;
+      }
+      if (++stage == g.stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    // Copies still in flight land before the ring is reused.
+    for (int i = 0; i < armed; ++i) {
+      if (--stage < 0) {
+        stage = g.stages - 1;
+        phase ^= 1u;
+      }
+      warp_wait(&full[stage], phase, wctx, kStatusTimeoutTeardown);
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    const uint32_t idesc = idesc_s8(kBlockM, g.bn);
+    const uint64_t a_desc0 = smem_desc(smem_u32(a_ring), 16, 8 * kBlockK, Layout::kSw128);
+    const uint64_t b_desc0 = smem_desc(smem_u32(b_ring), 16, 8 * kBlockK, Layout::kSw128);
+    const uint32_t a_step = plan.a_box >> 4;
+    const uint32_t b_step = plan.b_box >> 4;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb_begin; kb < kb_end; kb += kSub) {
+      if (!warp_wait(&full[stage], phase, wctx, kStatusTimeoutFull)) break;
+      tc_fence_after();
+      const int boxes = kb_end - kb < kSub ? kb_end - kb : kSub;
+      if (elect_one()) {
+#pragma unroll
+        for (int i = 0; i < kSub; ++i) {
+          if (i < boxes) {
+            const uint64_t ad = a_desc0 + (stage * kSub + i) * a_step;
+            const uint64_t bd = b_desc0 + (stage * kSub + i) * b_step;
+#pragma unroll
+            for (int k = 0; k < kBlockK / 32; ++k)
+              umma_i8(tmem_base, ad + 2 * k, bd + 2 * k, idesc, kb - kb_begin + i + k > 0 ? 1u : 0u);
+          }
+        }
+        umma_commit(&empty[stage]);
+      }
+      __syncwarp();
+      if (++stage == g.stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    // Also after a wait that ran out: every MMA issued finishes before the ring
+    // is reused and TMEM is released.
+    if (elect_one()) umma_commit(tfull);
+    __syncwarp();
+    warp_wait(tfull, 0, wctx, kStatusTimeoutTeardown);
+  } else {
+    // ---------------- partial sums to shared memory (warps 2..9) ----------------
+    griddep_wait();
+    if (warp == 2) griddep_launch_dependents();
+    const int quarter = warp & 3;
+    const int half = (warp - 2) >> 2;
+    if (warp_wait(tfull, 0, wctx, kStatusTimeoutAccum) && quarter * 32 < rows && kb_begin < kb_end) {
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+      for (int c0 = 32 * half; c0 < g.bn; c0 += 64) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(taddr + c0, v);
+        tmem_ld_wait();
+        if (quarter * 32 + lane < rows) {
+          int4 *dst = reinterpret_cast<int4 *>(partial + (quarter * 32 + lane) * pitch + c0);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            dst[j] = make_int4(static_cast<int32_t>(v[4 * j]), static_cast<int32_t>(v[4 * j + 1]),
+                               static_cast<int32_t>(v[4 * j + 2]), static_cast<int32_t>(v[4 * j + 3]));
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp >= 2) {
+    using T = typename Elem<OUT>::type;
+    const int wide = g.bn / g.splits / 4;                   // this CTA's columns, in fours
+    const int parts = (g.kblocks + share - 1) / share;      // CTAs that hold a partial sum
+    const uint32_t here = smem_u32(partial);
+    for (int i = static_cast<int>(threadIdx.x) - 64; i < rows * wide; i += kThreads - 64) {
+      const int r = i / wide, c = (rank * wide + i - r * wide) * 4;
+      const int row = m0 + r, col = n0 + c;
+      if (col >= g.N) continue;
+      const uint32_t at = here + (r * pitch + c) * 4;
+      int4 part[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        part[k] = k < parts ? ld_cluster_v4(mapa_shared(at, k)) : make_int4(0, 0, 0, 0);
+      float cs[4], b[4], res[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = col + j < g.N;
+        cs[j] = in && g.col_scale != nullptr ? __ldg(g.col_scale + col + j) : 1.f;
+        b[j] = in && g.bias != nullptr ? __ldg(g.bias + col + j) : 0.f;
+        res[j] = 0.f;
+        if constexpr (OUT != INT8CONV_INT8) {
+          if (in && g.residual != nullptr)
+            res[j] = Elem<OUT>::load(static_cast<const T *>(g.residual)[row * g.ldr + col + j]);
+        }
+      }
+      const float rs = g.row_scale != nullptr ? __ldg(g.row_scale + row) : 1.f;
+      int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        sum.x += part[k].x;
+        sum.y += part[k].y;
+        sum.z += part[k].z;
+        sum.w += part[k].w;
+      }
+      const int32_t acc[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float v = activate_any(fmaf(static_cast<float>(acc[j]) * cs[j], rs, b[j]), g.activation);
+        v = OUT == INT8CONV_INT8 ? v * g.inv_out_scale : v + res[j];
+        if (col + j < g.N) static_cast<T *>(g.y)[row * g.ldy + col + j] = Elem<OUT>::store(v);
+      }
+    }
+  }
+  // No CTA leaves while another may still read its partial sums.
+  cluster_sync_all();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, g.tmem_cols);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
@@ -713,6 +949,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 struct TileChoice {
   bool pair;
   int bn;
+  int splits;
 };
 
 // The candidate with the least estimated time, in cycles.  For each 128 bytes
@@ -724,10 +961,12 @@ struct TileChoice {
 // were fitted to 20 plain and grouped shapes timed at every width, single and
 // in pairs: the choice is within 3 % of the fastest on each (2048 x 4096 x 4096:
 // pairs of 256 columns 27.7 us, best of 15 27.7, worst 69; 32768 x 320 x 320:
-// single, 160 columns, 11.9 us, worst 21.6).
+// single, 160 columns, 11.9 us, worst 21.6).  Few tiles may also share k (the
+// split kernel): 1 x 4096 x 4096 in 4 shares of 128 columns 5.9 us, unsplit 7.0;
+// 8 x 4096 x 16384 10.3 and 20.5; 128 x 4096 x 4096 9.4 and 7.4 (unsplit taken).
 TileChoice choose_tile(double row_tiles128, double row_tiles256, int64_t n, int kblocks, int a_rows,
-                       int sms) {
-  TileChoice best{false, 128};
+                       int sms, int rows, bool split) {
+  TileChoice best{false, 128, 1};
   double best_cost = 1e300;
   auto consider = [&](bool pair, int bn) {
     const double tiles = (pair ? row_tiles256 : row_tiles128) * static_cast<double>((n + bn - 1) / bn);
@@ -740,7 +979,7 @@ TileChoice choose_tile(double row_tiles128, double row_tiles256, int64_t n, int 
                         (pair ? 1000.0 : 0.0);
     if (cost < best_cost) {
       best_cost = cost;
-      best = TileChoice{pair, bn};
+      best = TileChoice{pair, bn, 1};
     }
   };
   if (a_rows == kBlockM && pairing_mode() != 1) {
@@ -748,6 +987,25 @@ TileChoice choose_tile(double row_tiles128, double row_tiles256, int64_t n, int 
     if (pairing_mode() == 2) return best;
   }
   for (int bn = 256; bn >= 32; bn -= 32) consider(false, bn);
+  if (split && pairing_mode() == 0) {
+    // Shares of k, where all clusters run at one time.
+    const int32_t clusters[9] = I8C_B200_CLUSTERS;
+    for (int splits = 2; splits <= 8; splits *= 2) {
+      for (int bn = 256; bn >= 64; bn -= 64) {
+        if (row_tiles128 * static_cast<double>((n + bn - 1) / bn) > clusters[splits]) continue;
+        const int share = (kblocks + 2 * splits - 1) / (2 * splits) * 2;
+        const double box = fmax(fmax(2.0 * bn, (a_rows + bn) * (kBlockK / 80.0)), 285.0);
+        // Cluster launch and barriers, more of them for 8 CTAs, and the sums:
+        // 16 bytes from each of the CTAs for 1024 values at a time.
+        const double cost = share * box + (splits == 8 ? 4500.0 : 2500.0) +
+                            1200.0 * ceil(rows * bn / (1024.0 * splits));
+        if (cost < best_cost) {
+          best_cost = cost;
+          best = TileChoice{false, bn, splits};
+        }
+      }
+    }
+  }
   return best;
 }
 
@@ -814,6 +1072,19 @@ const void *kernel_for(int dtype) {
   }
 }
 
+const void *split_kernel_for(int dtype) {
+  switch (dtype) {
+    case INT8CONV_BF16:
+      return reinterpret_cast<const void *>(&matmul_split_kernel<INT8CONV_BF16>);
+    case INT8CONV_FP16:
+      return reinterpret_cast<const void *>(&matmul_split_kernel<INT8CONV_FP16>);
+    case INT8CONV_FP32:
+      return reinterpret_cast<const void *>(&matmul_split_kernel<INT8CONV_FP32>);
+    default:
+      return reinterpret_cast<const void *>(&matmul_split_kernel<INT8CONV_INT8>);
+  }
+}
+
 bool aligned(const void *p, int64_t bytes) {
   return (reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes)) == 0;
 }
@@ -848,7 +1119,7 @@ int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, co
     while (g.box_rows > 8 && g.box_rows > each) g.box_rows /= 2;
   }
   const TileChoice c = choose_tile(row_tiles(kBlockM), row_tiles(2 * kBlockM), d.n, g.kblocks,
-                                   g.box_rows, sms);
+                                   g.box_rows, sms, g.M < kBlockM ? g.M : kBlockM, !grouped);
   g.bn = c.bn;
   const int tile_rows = c.pair ? 2 * kBlockM : kBlockM;
   g.n_tiles = static_cast<int32_t>((d.n + g.bn - 1) / g.bn);
@@ -891,6 +1162,25 @@ int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, co
   if (g.tma_store && !result_map(&tmap_y, y, d.y_dtype, d.m, d.n, d.ldy)) return INT8CONV_CUDA_ERROR;
 
   LaunchPlan plan;
+  if (c.splits > 1) {
+    g.splits = c.splits;
+    g.tmem_cols = 32;
+    while (g.tmem_cols < g.bn) g.tmem_cols *= 2;
+    plan.func = split_kernel_for(d.y_dtype);
+    // The partial sums take the place of the ring, with which the largest tile
+    // of them (128 rows x 256 columns, 130 KB) always fits.
+    const MatmulSmem layout = matmul_smem(g.a_rows, g.bn, g.stages, 0);
+    const uint32_t sums = static_cast<uint32_t>(g.M < kBlockM ? g.M : kBlockM) * (g.bn + 4) * 4;
+    if (sums > layout.bar_off) return INT8CONV_CUDA_ERROR;
+    plan.smem = layout.total;
+    if (plan.smem < kMaxSmem / 2 + 1024) plan.smem = kMaxSmem / 2 + 1024;
+    if (!ensure_smem_attr(plan.func, static_cast<int>(plan.smem))) return INT8CONV_CUDA_ERROR;
+    plan.cluster = static_cast<uint32_t>(c.splits);
+    plan.grid = dim3(static_cast<unsigned>(g.m_tiles * g.n_tiles * c.splits));
+    plan.block = dim3(kThreads);
+    plan_args(plan, tmap_a, tmap_b, g, run_ctl());
+    return launch_plan(plan, stream);
+  }
   plan.func = c.pair ? (grouped ? kernel_for<true, true>(d.y_dtype) : kernel_for<true, false>(d.y_dtype))
                      : (grouped ? kernel_for<false, true>(d.y_dtype) : kernel_for<false, false>(d.y_dtype));
   plan.smem = smem_of(g.stages);

@@ -63,7 +63,8 @@ def pairing(request):
 
 SHAPES = [(1, 1, 1), (1, 4096, 512), (2, 33, 16), (3, 5, 7), (8, 1000, 2050), (16, 64, 4096),
           (17, 96, 100), (65, 31, 129), (128, 256, 128), (129, 257, 131), (200, 1000, 1040),
-          (513, 640, 96), (1100, 2100, 260)]
+          (513, 640, 96), (1100, 2100, 260), (1, 500, 4100), (100, 300, 5000),
+          (3, 70, 16400), (128, 512, 1536), (140, 200, 3000)]
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=str)
