@@ -71,6 +71,15 @@ struct Raw8 {
   __device__ __forceinline__ float get(int j) const {
     return Elem<DT>::load(reinterpret_cast<const T *>(w)[j]);
   }
+  // Elements j and j + 1 (j even) as an fp32 pair.
+  __device__ __forceinline__ uint64_t pair(int j) const {
+    if constexpr (DT == INT8CONV_BF16) {
+      const uint32_t u = reinterpret_cast<const uint32_t *>(w)[j >> 1];
+      return f2_pack(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    } else {
+      return f2_pack(get(j), get(j + 1));
+    }
+  }
   // The larger of `top` and the bits of every |x|; 16-bit types two at a time,
   // each half on its own.
   __device__ __forceinline__ uint32_t max_bits(uint32_t top) const {
@@ -88,8 +97,15 @@ struct Raw8 {
   }
 };
 
+// CTAs that an SM should hold at one time: rows on their way hide the latency of
+// index, row and reduction.  fp32 rows take twice the registers.
 template <int DT, int WARPS>
-__global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS)
+constexpr int block_count() {
+  return (DT == INT8CONV_FP32 ? 1024 : 1536) / (WARPS < 4 ? 128 : 32 * WARPS);
+}
+
+template <int DT, int WARPS>
+__global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS, block_count<DT, WARPS>())
     quantize_kernel(const QuantizeArgs a) {
   using T = typename Elem<DT>::type;
   constexpr int kThreads = WARPS < 4 ? 128 : 32 * WARPS;
@@ -145,19 +161,27 @@ __global__ void __launch_bounds__(WARPS < 4 ? 128 : 32 * WARPS)
   const bool divide = scale < 7.8886090522101181e-31f;
   const float inv = zero ? 0.f : __frcp_rn(scale);
   auto put = [&](int64_t k0, const Raw8<DT> &f) {
+    // Adding 1.5 * 2^23 rounds to an integer, half to even, whose low byte is
+    // the sum's.
+    const uint64_t inv2 = f2_pack(inv, inv);
+    const uint64_t magic = f2_pack(12582912.f, 12582912.f);
+    const uint64_t minus = f2_pack(-12582912.f, -12582912.f);
+    const uint64_t negate = f2_pack(-1.f, -1.f);
     uint32_t w[2];
     float near = 0.f;   // largest distance from an integer
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t b[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        // Adding 1.5 * 2^23 rounds to an integer, half to even, whose low byte
-        // is the sum's.
-        const float p = f.get(4 * h + j) * inv;
-        const float t = p + 12582912.f;
-        near = fmaxf(near, fabsf(p - (t - 12582912.f)));
-        b[j] = __float_as_uint(t);
+      for (int j = 0; j < 4; j += 2) {
+        const uint64_t p = f2_mul(f.pair(4 * h + j), inv2);
+        const uint64_t s = f2_add(p, magic);
+        float lo, hi;
+        f2_unpack(f2_fma(f2_add(s, minus), negate, p), lo, hi);
+        near = fmaxf(near, fmaxf(fabsf(lo), fabsf(hi)));
+        f2_unpack(s, lo, hi);
+        b[j] = __float_as_uint(lo);
+        b[j + 1] = __float_as_uint(hi);
       }
       w[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     }
