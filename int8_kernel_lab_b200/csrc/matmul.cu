@@ -56,6 +56,11 @@ constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kTableBytes = 1024;             // 128 columns x (scale, bias) per warp
 constexpr int kMaxStages = 14;
 
+// Forms of the kernel.
+constexpr int kPlain = 0;
+constexpr int kGrouped = 1;     // rows grouped by expert
+constexpr int kResidentB = 2;   // a CTA's column tile of B stays in shared memory
+
 struct MatmulGeom {
   int32_t M, N;
   int32_t kblocks;     // boxes of 128 bytes of k
@@ -99,16 +104,20 @@ struct MatmulSmem {
   uint32_t b_off, staging_off, table_off, bar_off, group_off, total;
 };
 
-__host__ __device__ inline MatmulSmem matmul_smem(int a_rows, int b_rows, int stages, int groups) {
+// `resident`: boxes of B that stay in shared memory for the whole launch, instead
+// of B's share of the ring.
+__host__ __device__ inline MatmulSmem matmul_smem(int a_rows, int b_rows, int stages, int groups,
+                                                  int resident) {
   MatmulSmem p;
   p.a_box = a_rows * kBlockK;
   p.b_box = b_rows * kBlockK;
   p.b_off = stages * kSub * p.a_box;
-  p.staging_off = p.b_off + stages * kSub * p.b_box;   // boxes are multiples of 1024 bytes
+  // Boxes are multiples of 1024 bytes.
+  p.staging_off = p.b_off + (resident > 0 ? resident : stages * kSub) * p.b_box;
   p.table_off = p.staging_off + kEpiWarps * kStageBytes;
   p.bar_off = p.table_off + kEpiWarps * kTableBytes;
-  // full/empty[stages], tfull[2], tempty[2], drain, TMEM slot
-  p.group_off = p.bar_off + (2 * stages + 5) * 8 + 8;
+  // full/empty[stages], tfull[2], tempty[2], drain, resident B, TMEM slot
+  p.group_off = p.bar_off + (2 * stages + 6) * 8 + 8;
   p.total = 1024 + p.group_off + (groups > 0 ? (2 * groups + 2) * 4 : 0);
   return p;
 }
@@ -123,11 +132,16 @@ struct Tile {
 // Work units of a launch.  Plain: bands of `band` row tiles, and inside a band
 // column by column, so that the CTAs running at one time share few rows of A
 // and of B.  Grouped: expert by expert, column by column.
-template <bool GROUPED>
+template <int MODE>
 __device__ __forceinline__ Tile tile_at(const MatmulGeom &g, int tile_rows, const int32_t *row_start,
                                         const int32_t *tile_start, int u) {
   Tile t;
-  if constexpr (GROUPED) {
+  if constexpr (MODE == kResidentB) {
+    t.group = 0;
+    t.m0 = u / g.n_tiles * tile_rows;
+    t.m_end = g.M;
+    t.n0 = u % g.n_tiles * g.bn;
+  } else if constexpr (MODE == kGrouped) {
     int lo = 0, hi = g.groups;   // tile_start[lo] * n_tiles <= u < tile_start[hi] * n_tiles
     const int at = u / g.n_tiles;
     while (hi - lo > 1) {
@@ -315,7 +329,7 @@ __device__ __forceinline__ void copy_out(const uint4 *stg, typename Elem<OUT>::t
   }
 }
 
-template <bool PAIR, bool GROUPED, int OUT>
+template <bool PAIR, int MODE, int OUT>
 __global__ void __launch_bounds__(kThreads, 1)
     matmul_kernel(const __grid_constant__ CUtensorMap tmap_a,
                   const __grid_constant__ CUtensorMap tmap_b,
@@ -326,9 +340,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   // of a pair.
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  constexpr bool GROUPED = MODE == kGrouped, RESIDENT = MODE == kResidentB;
+  static_assert(!(PAIR && RESIDENT), "resident B runs single CTAs");
   constexpr int kTileRows = PAIR ? 2 * kBlockM : kBlockM;
   const MatmulSmem plan = matmul_smem(g.a_rows, PAIR ? g.bn / 2 : g.bn, g.stages,
-                                      GROUPED ? g.groups : 0);
+                                      GROUPED ? g.groups : 0, RESIDENT ? g.kblocks : 0);
   uint8_t *a_ring = smem;
   uint8_t *b_ring = smem + plan.b_off;
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + plan.bar_off);
@@ -336,7 +352,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t *tfull = empty + g.stages;
   uint64_t *tempty = tfull + 2;
   uint64_t *drain = tempty + 2;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+  uint64_t *b_here = drain + 1;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(b_here + 1);
   int32_t *row_start = reinterpret_cast<int32_t *>(smem + plan.group_off);
   int32_t *tile_start = row_start + g.groups + 1;
 
@@ -349,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int step = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
 
   if (warp == 0) {
-    for (int i = lane; i < 2 * g.stages + 5; i += 32) {
+    for (int i = lane; i < 2 * g.stages + 6; i += 32) {
       // tempty: one arrival per epilogue warp (of both CTAs for a pair).
       const bool te = i >= 2 * g.stages + 2 && i < 2 * g.stages + 4;
       mbar_init(&full[i], te ? (PAIR ? 2 : 1) * kEpiWarps : 1);
@@ -422,9 +439,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t phase = 0;
     int armed = 0;
     const uint32_t box_bytes = static_cast<uint32_t>(g.box_rows * kBlockK);
+    if constexpr (RESIDENT) {
+      if (!ctl.starve) {
+        const int n0 = first % g.n_tiles * g.bn;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(b_here, g.kblocks * plan.b_box);
+          for (int kb = 0; kb < g.kblocks; ++kb)
+            tma_load_3d(b_ring + kb * plan.b_box, &tmap_b, b_here, kb * kBlockK, n0, 0);
+        }
+        __syncwarp();
+      }
+    }
     bool ok = true;
     for (int u = first; u < num_tiles && ok; u += step) {
-      const Tile t = tile_at<GROUPED>(g, kTileRows, row_start, tile_start, u);
+      const Tile t = tile_at<MODE>(g, kTileRows, row_start, tile_start, u);
       const int m0 = t.m0 + static_cast<int>(rank) * kBlockM;
       const int n0 = t.n0 + static_cast<int>(rank) * (PAIR ? g.bn / 2 : 0);
       // A plain product's boxes cover the tile; a group's as many as its rows need.
@@ -433,7 +461,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int rows = t.m_end - m0 < g.a_rows ? t.m_end - m0 : g.a_rows;
         parts = __shfl_sync(0xffffffffu, (rows + g.box_rows - 1) / g.box_rows, 0);
       }
-      const uint32_t tx = (PAIR ? 2u : 1u) * (parts * box_bytes + plan.b_box);   // 128 bytes of k
+      // Bytes of 128 bytes of k.
+      const uint32_t tx = (PAIR ? 2u : 1u) * (parts * box_bytes + (RESIDENT ? 0 : plan.b_box));
       for (int kb = 0; kb < g.kblocks; kb += kSub) {
         if (!warp_wait(&empty[stage], phase ^ 1u, wctx, kStatusTimeoutEmpty)) {
           ok = false;
@@ -458,8 +487,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                   for (int j = 0; j < parts; ++j)
                     tma_load_3d(adst + i * plan.a_box + j * box_bytes, &tmap_a, &full[stage],
                                 (kb + i) * kBlockK, m0 + j * g.box_rows, 0);
-                  tma_load_3d(bdst + i * plan.b_box, &tmap_b, &full[stage], (kb + i) * kBlockK, n0,
-                              t.group);
+                  if constexpr (!RESIDENT)
+                    tma_load_3d(bdst + i * plan.b_box, &tmap_b, &full[stage], (kb + i) * kBlockK,
+                                n0, t.group);
                 }
               }
             }
@@ -482,6 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       warp_wait(&full[stage], phase, wctx, kStatusTimeoutTeardown);
     }
+    if (RESIDENT && !ctl.starve) warp_wait(b_here, 0, wctx, kStatusTimeoutTeardown);
   } else if (warp == 1) {
     if (leader) {
       // ---------------- MMA issuer (the leader of a pair) ----------------
@@ -493,6 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
+      if constexpr (RESIDENT) ok = warp_wait(b_here, 0, wctx, kStatusTimeoutFull);
       for (int u = first; u < num_tiles && ok; u += step) {
         if (!warp_wait(&tempty[acc], acc_phase ^ 1u, wctx, kStatusTimeoutDrain)) break;
         tc_fence_after();
@@ -509,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < kSub; ++i) {
               if (i < boxes) {
                 const uint64_t ad = a_desc0 + (stage * kSub + i) * a_step;
-                const uint64_t bd = b_desc0 + (stage * kSub + i) * b_step;
+                const uint64_t bd = b_desc0 + (RESIDENT ? kb + i : stage * kSub + i) * b_step;
 #pragma unroll
                 for (int k = 0; k < kBlockK / 32; ++k) {
                   const uint32_t accumulate = kb + i + k > 0 ? 1u : 0u;
@@ -561,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t acc_phase = 0;
     int table_n0 = -1, table_group = -1;
     for (int u = first; u < num_tiles; u += step) {
-      const Tile t = tile_at<GROUPED>(g, kTileRows, row_start, tile_start, u);
+      const Tile t = tile_at<MODE>(g, kTileRows, row_start, tile_start, u);
       const int row0 = t.m0 + static_cast<int>(rank) * kBlockM + quarter * 32;
       const int rows = t.m_end - row0;        // rows of this warp's 32 that count (may be <= 0)
       const bool mine = lane < rows;
@@ -748,14 +780,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  const MatmulSmem plan = matmul_smem(g.a_rows, g.bn, g.stages, 0);
+  const MatmulSmem plan = matmul_smem(g.a_rows, g.bn, g.stages, 0, 0);
   uint8_t *a_ring = smem;
   uint8_t *b_ring = smem + plan.b_off;
   int32_t *partial = reinterpret_cast<int32_t *>(smem);
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + plan.bar_off);
   uint64_t *empty = full + g.stages;
   uint64_t *tfull = empty + g.stages;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tfull + 5);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tfull + 6);
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0);   // uniform
   const int lane = threadIdx.x & 31;
   const WaitCtx wctx{ctl.wait_ns, ctl.status};
@@ -950,36 +982,38 @@ struct TileChoice {
   bool pair;
   int bn;
   int splits;
+  bool resident;
 };
 
 // The candidate with the least estimated time, in cycles.  For each 128 bytes
 // of k a CTA's tensor core needs 2 * bn (128 x bn x 32 bytes in bn / 2; a pair
 // 256 x bn in the same), its loads (a_rows rows of A and its share of B, 128
-// bytes each) come at about 80 bytes a cycle, and the issuer needs 285; the
-// slowest counts.  The epilogue of the tile before runs meanwhile.  A pair
-// loses about 2500 cycles between two tiles and 1000 at the start.  The rates
-// were fitted to 20 plain and grouped shapes timed at every width, single and
-// in pairs: the choice is within 3 % of the fastest on each (2048 x 4096 x 4096:
+// bytes each) come at about 72 bytes a cycle, and the issuer needs 285; the
+// slowest counts.  The epilogue of the tile before runs meanwhile, 5 cycles a
+// column and 400 for its latencies.  A pair loses about 2500 cycles between two
+// tiles and 3000 at the start.  The rates were fitted to 28 plain and grouped
+// shapes timed at every width, single, in pairs and with resident B: the choice
+// is within 5 % of the fastest on each, within 1 % on most (2048 x 4096 x 4096:
 // pairs of 256 columns 27.7 us, best of 15 27.7, worst 69; 32768 x 320 x 320:
-// single, 160 columns, 11.9 us, worst 21.6).  Few tiles may also share k (the
+// resident, 160 columns, 11.0 us, not resident 11.9, worst 21.6).  Few tiles may also share k (the
 // split kernel): 1 x 4096 x 4096 in 4 shares of 128 columns 5.9 us, unsplit 7.0;
 // 8 x 4096 x 16384 10.3 and 20.5; 128 x 4096 x 4096 9.4 and 7.4 (unsplit taken).
 TileChoice choose_tile(double row_tiles128, double row_tiles256, int64_t n, int kblocks, int a_rows,
-                       int sms, int rows, bool split) {
-  TileChoice best{false, 128, 1};
+                       int sms, int rows, bool grouped) {
+  TileChoice best{false, 128, 1, false};
   double best_cost = 1e300;
   auto consider = [&](bool pair, int bn) {
     const double tiles = (pair ? row_tiles256 : row_tiles128) * static_cast<double>((n + bn - 1) / bn);
     const double waves = ceil(tiles / (pair ? sms / 2 : sms) - 1e-9);
     const double mma = 2.0 * bn;
-    const double load = (a_rows + (pair ? bn / 2 : bn)) * (kBlockK / 80.0);
+    const double load = (a_rows + (pair ? bn / 2 : bn)) * (kBlockK / 72.0);
     const double box = fmax(fmax(mma, load), 285.0);
-    const double finish = 5.0 * bn;
+    const double finish = 400.0 + 5.0 * bn;
     const double cost = waves * (fmax(kblocks * box, finish) + (pair ? 2500.0 : 100.0)) + finish +
-                        (pair ? 1000.0 : 0.0);
+                        (pair ? 3000.0 : 0.0);
     if (cost < best_cost) {
       best_cost = cost;
-      best = TileChoice{pair, bn, 1};
+      best = TileChoice{pair, bn, 1, false};
     }
   };
   if (a_rows == kBlockM && pairing_mode() != 1) {
@@ -987,21 +1021,39 @@ TileChoice choose_tile(double row_tiles128, double row_tiles256, int64_t n, int 
     if (pairing_mode() == 2) return best;
   }
   for (int bn = 256; bn >= 32; bn -= 32) consider(false, bn);
-  if (split && pairing_mode() == 0) {
+  if (!grouped && pairing_mode() == 0 && a_rows == kBlockM) {
+    // A column tile of B that stays: only A is loaded for each row tile.
+    for (int bn = 256; bn >= 32; bn -= 32) {
+      const int64_t n_tiles = (n + bn - 1) / bn;
+      if (n_tiles > sms ||
+          matmul_smem(kBlockM, bn, 3, 0, kblocks).total > static_cast<uint32_t>(kMaxSmem))
+        continue;
+      const double waves = ceil(row_tiles128 / static_cast<double>(sms / n_tiles) - 1e-9);
+      const double box = fmax(fmax(2.0 * bn, kBlockM * (kBlockK / 72.0)), 285.0);
+      const double finish = 400.0 + 5.0 * bn;
+      const double cost = waves * (fmax(kblocks * box, finish) + 100.0) + finish +
+                          kblocks * bn * (kBlockK / 72.0);
+      if (waves > 1.0 && cost < best_cost) {
+        best_cost = cost;
+        best = TileChoice{false, bn, 1, true};
+      }
+    }
+  }
+  if (!grouped && pairing_mode() == 0) {
     // Shares of k, where all clusters run at one time.
     const int32_t clusters[9] = I8C_B200_CLUSTERS;
     for (int splits = 2; splits <= 8; splits *= 2) {
       for (int bn = 256; bn >= 64; bn -= 64) {
         if (row_tiles128 * static_cast<double>((n + bn - 1) / bn) > clusters[splits]) continue;
         const int share = (kblocks + 2 * splits - 1) / (2 * splits) * 2;
-        const double box = fmax(fmax(2.0 * bn, (a_rows + bn) * (kBlockK / 80.0)), 285.0);
+        const double box = fmax(fmax(2.0 * bn, (a_rows + bn) * (kBlockK / 72.0)), 285.0);
         // Cluster launch and barriers, more of them for 8 CTAs, and the sums:
         // 16 bytes from each of the CTAs for 1024 values at a time.
         const double cost = share * box + (splits == 8 ? 4500.0 : 2500.0) +
                             1200.0 * ceil(rows * bn / (1024.0 * splits));
         if (cost < best_cost) {
           best_cost = cost;
-          best = TileChoice{false, bn, splits};
+          best = TileChoice{false, bn, splits, false};
         }
       }
     }
@@ -1058,17 +1110,17 @@ bool result_map(CUtensorMap *map, void *y, int dtype, int64_t m, int64_t n, int6
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool PAIR, bool GROUPED>
+template <bool PAIR, int MODE>
 const void *kernel_for(int dtype) {
   switch (dtype) {
     case INT8CONV_BF16:
-      return reinterpret_cast<const void *>(&matmul_kernel<PAIR, GROUPED, INT8CONV_BF16>);
+      return reinterpret_cast<const void *>(&matmul_kernel<PAIR, MODE, INT8CONV_BF16>);
     case INT8CONV_FP16:
-      return reinterpret_cast<const void *>(&matmul_kernel<PAIR, GROUPED, INT8CONV_FP16>);
+      return reinterpret_cast<const void *>(&matmul_kernel<PAIR, MODE, INT8CONV_FP16>);
     case INT8CONV_FP32:
-      return reinterpret_cast<const void *>(&matmul_kernel<PAIR, GROUPED, INT8CONV_FP32>);
+      return reinterpret_cast<const void *>(&matmul_kernel<PAIR, MODE, INT8CONV_FP32>);
     default:
-      return reinterpret_cast<const void *>(&matmul_kernel<PAIR, GROUPED, INT8CONV_INT8>);
+      return reinterpret_cast<const void *>(&matmul_kernel<PAIR, MODE, INT8CONV_INT8>);
   }
 }
 
@@ -1119,7 +1171,7 @@ int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, co
     while (g.box_rows > 8 && g.box_rows > each) g.box_rows /= 2;
   }
   const TileChoice c = choose_tile(row_tiles(kBlockM), row_tiles(2 * kBlockM), d.n, g.kblocks,
-                                   g.box_rows, sms, g.M < kBlockM ? g.M : kBlockM, !grouped);
+                                   g.box_rows, sms, g.M < kBlockM ? g.M : kBlockM, grouped);
   g.bn = c.bn;
   const int tile_rows = c.pair ? 2 * kBlockM : kBlockM;
   g.n_tiles = static_cast<int32_t>((d.n + g.bn - 1) / g.bn);
@@ -1133,7 +1185,7 @@ int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, co
   while (g.tmem_cols < 2 * g.bn) g.tmem_cols *= 2;
   const int b_rows = c.pair ? g.bn / 2 : g.bn;
   const auto smem_of = [&](int stages) {
-    return matmul_smem(g.a_rows, b_rows, stages, groups).total;
+    return matmul_smem(g.a_rows, b_rows, stages, groups, c.resident ? g.kblocks : 0).total;
   };
   g.stages = kMaxStages;
   while (g.stages > 2 && smem_of(g.stages) > static_cast<uint32_t>(kMaxSmem)) --g.stages;
@@ -1169,7 +1221,7 @@ int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, co
     plan.func = split_kernel_for(d.y_dtype);
     // The partial sums take the place of the ring, with which the largest tile
     // of them (128 rows x 256 columns, 130 KB) always fits.
-    const MatmulSmem layout = matmul_smem(g.a_rows, g.bn, g.stages, 0);
+    const MatmulSmem layout = matmul_smem(g.a_rows, g.bn, g.stages, 0, 0);
     const uint32_t sums = static_cast<uint32_t>(g.M < kBlockM ? g.M : kBlockM) * (g.bn + 4) * 4;
     if (sums > layout.bar_off) return INT8CONV_CUDA_ERROR;
     plan.smem = layout.total;
@@ -1181,8 +1233,11 @@ int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, co
     plan_args(plan, tmap_a, tmap_b, g, run_ctl());
     return launch_plan(plan, stream);
   }
-  plan.func = c.pair ? (grouped ? kernel_for<true, true>(d.y_dtype) : kernel_for<true, false>(d.y_dtype))
-                     : (grouped ? kernel_for<false, true>(d.y_dtype) : kernel_for<false, false>(d.y_dtype));
+  plan.func = c.pair      ? (grouped ? kernel_for<true, kGrouped>(d.y_dtype)
+                                     : kernel_for<true, kPlain>(d.y_dtype))
+              : grouped    ? kernel_for<false, kGrouped>(d.y_dtype)
+              : c.resident ? kernel_for<false, kResidentB>(d.y_dtype)
+                           : kernel_for<false, kPlain>(d.y_dtype);
   plan.smem = smem_of(g.stages);
   // At least half an SM's shared memory: one CTA per SM, so that none waits
   // for another's TMEM columns.
@@ -1191,7 +1246,7 @@ int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, co
   if (!ensure_smem_attr(plan.func, static_cast<int>(plan.smem))) return INT8CONV_CUDA_ERROR;
   plan.cluster = c.pair ? 2 : 1;
   const int64_t tiles = m_tiles * g.n_tiles;
-  const int64_t slots = c.pair ? sms / 2 : sms;
+  const int64_t slots = c.pair ? sms / 2 : c.resident ? sms / g.n_tiles * g.n_tiles : sms;
   plan.grid = dim3(static_cast<unsigned>((tiles < slots ? tiles : slots) * plan.cluster));
   plan.block = dim3(kThreads);
   plan_args(plan, tmap_a, tmap_b, tmap_y, g, run_ctl());
