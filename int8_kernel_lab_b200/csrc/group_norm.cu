@@ -21,6 +21,7 @@
 #include <math.h>
 
 #include "epilogue.cuh"
+#include "int8conv_rules.h"
 #include "launch.h"
 #include "sm100.cuh"
 
@@ -627,17 +628,20 @@ NormShape norm_shape(const int8conv_group_norm &d) {
   // for each SM (measured, us: 32 images of 196 x 512 bf16 in clusters of 1 / 4 /
   // 8: 15.6 / 9.6 / 11.1; 64 of 3136 x 256 int32: 191 / 86 / 90).  16 CTAs never
   // pay: at most 7 such clusters find room on the GPU at one time.
-  const int64_t want = d.n * bytes < (16 << 20) ? 128 : 256;
+  const int64_t total = d.n * bytes;
+  const int64_t want = total < (16 << 20) ? 128 : 256;
   int spans = 1;
   while (spans < kMaxCluster && d.n * spans < want && bytes > spans * int64_t(8 * 1024)) spans *= 2;
   if (spans > d.pixels) spans = 1;
   NormShape s{true, spans, (d.pixels + spans - 1) / spans};
-  // Few images with more than 32 KB for each CTA of such a cluster: two kernels
-  // over chunks of all images, one CTA for each SM, or two where each still has
-  // 128 KB (8 images of 4096 x 320 bf16: 19.2 us, in clusters of 8 28.4;
-  // 1 image: 9.9 and 24.6).
-  if (d.n * spans < 96 && bytes > spans * int64_t(32 * 1024)) {
-    const int64_t all = d.n * bytes > 148 * int64_t(128 * 1024) ? 296 : 148;
+  // Few images with much for each CTA of such a cluster: two kernels over chunks
+  // of all images, one to four for each SM by what there is to read (8 images of
+  // 4096 x 320 bf16: 19.2 us, in clusters of 8 28.4; 1 image 9.9 and 24.6; 16 of
+  // 8192 x 256 50 and 91; but 10 of 1400 x 112 10.4 and 8.4, 32 of 4096 x 512
+  // 100 and 83).
+  const int64_t each = bytes / spans;
+  if ((d.n * spans < 96 && each > 64 * 1024) || (d.n * spans <= 148 && each > 256 * 1024)) {
+    const int64_t all = total > (64 << 20) ? 592 : total > (19 << 20) ? 296 : 148;
     int64_t chunks = (all + d.n - 1) / d.n;
     if (chunks > d.pixels) chunks = d.pixels;
     s.cluster = false;
@@ -706,9 +710,10 @@ int8conv_status launch_group_norm_impl(const int8conv_group_norm &d, const void 
       need += (shape.span_pixels + lanes - 1) / lanes;
     }
     const uint32_t base = norm_smem(width, xs, d.channels, d.groups, 0).total;
-    // A grid of at most one CTA per SM takes more than half an SM's shared
-    // memory, so that no two of them land on the same one.
-    const bool alone = d.n * shape.spans <= device_info().sm_count;
+    // Clusters that all find room with one CTA for each SM take more than half
+    // an SM's shared memory, so that no two CTAs land on the same one.
+    const int32_t clusters[9] = I8C_B200_CLUSTERS;
+    const bool alone = d.n <= clusters[shape.spans];
     const uint32_t limit = alone ? kMaxSmem : kHalfSmem;
     const int64_t room =
         base < limit ? (limit - base) / static_cast<uint32_t>(kThreads * width * xs) : 0;
