@@ -218,7 +218,8 @@ typedef enum int8conv_activation {
  * y and residual need the alignment of their elements only; 16-byte aligned
  * rows are stored faster.  residual has y's type; it may be y itself (same
  * address and pitch: y += ...), any other overlap is undefined.  Nothing
- * outside y's m x n elements is written. */
+ * outside y's m x n elements is written.  An infinity times a zero, or minus
+ * infinity through SILU or a GELU, is NaN, as in the formulas. */
 typedef struct int8conv_matmul {
   int64_t m, n, k;
   int64_t lda, ldb, ldy, ldr;
@@ -234,7 +235,7 @@ typedef struct int8conv_matmul {
 /* m = 0 or n = 0 is OK and writes nothing.  BAD_ARGUMENT for a negative size,
  * k outside [1, INT8CONV_MAX_PRODUCT_K], a pitch below the row or (lda, ldb)
  * not a multiple of 16, an unknown type or activation, a residual with INT8
- * output, or a bad out_scale; BAD_POINTER for a NULL operand or output, a or b
+ * output, a bad out_scale, or more than 2^30 tiles of output; BAD_POINTER for a NULL operand or output, a or b
  * not 16-byte aligned, or another buffer not aligned to its elements. */
 int8conv_status int8conv_launch_matmul(const int8conv_matmul *desc, const int8_t *a,
                                        const int8_t *b, void *y, void *stream);

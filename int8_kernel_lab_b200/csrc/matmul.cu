@@ -431,10 +431,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   if constexpr (GROUPED) num_tiles = tile_start[g.groups] * g.n_tiles;
+  // Nothing touches global memory, and no wait's limit starts to count, before
+  // the previous kernel in the stream is complete.
+  if constexpr (!GROUPED) griddep_wait();
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
-    if constexpr (!GROUPED) griddep_wait();
     int stage = 0;
     uint32_t phase = 0;
     int armed = 0;
@@ -578,7 +580,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---------------- epilogue (warps 2..9) ----------------
     using T = typename Elem<OUT>::type;
-    if constexpr (!GROUPED) griddep_wait();
     if (warp == 2) griddep_launch_dependents();
     const int quarter = warp & 3;           // TMEM lane quarter this warp may access
     const int half = (warp - 2) >> 2;       // 32-column blocks half, half + 2, ...
@@ -818,10 +819,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  // Nothing touches global memory, and no wait's limit starts to count, before
+  // the previous kernel in the stream is complete.
+  griddep_wait();
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
-    griddep_wait();
     int stage = 0, armed = 0;
     uint32_t phase = 0;
     for (int kb = kb_begin; kb < kb_end; kb += kSub) {
@@ -895,7 +898,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     warp_wait(tfull, 0, wctx, kStatusTimeoutTeardown);
   } else {
     // ---------------- partial sums to shared memory (warps 2..9) ----------------
-    griddep_wait();
     if (warp == 2) griddep_launch_dependents();
     const int quarter = warp & 3;
     const int half = (warp - 2) >> 2;
@@ -995,9 +997,10 @@ struct TileChoice {
 // shapes timed at every width, single, in pairs and with resident B: the choice
 // is within 5 % of the fastest on each, within 1 % on most (2048 x 4096 x 4096:
 // pairs of 256 columns 27.7 us, best of 15 27.7, worst 69; 32768 x 320 x 320:
-// resident, 160 columns, 11.0 us, not resident 11.9, worst 21.6).  Few tiles may also share k (the
-// split kernel): 1 x 4096 x 4096 in 4 shares of 128 columns 5.9 us, unsplit 7.0;
-// 8 x 4096 x 16384 10.3 and 20.5; 128 x 4096 x 4096 9.4 and 7.4 (unsplit taken).
+// resident, 160 columns, 11.0 us, not resident 11.9, worst 21.6).  Few tiles may
+// also share k (the split kernel): 1 x 4096 x 4096 in 4 shares of 128 columns
+// 5.9 us, unsplit 7.0; 8 x 4096 x 16384 10.3 and 20.5; 128 x 4096 x 4096 9.4 and
+// 7.4 (unsplit taken).
 TileChoice choose_tile(double row_tiles128, double row_tiles256, int64_t n, int kblocks, int a_rows,
                        int sms, int rows, bool grouped) {
   TileChoice best{false, 128, 1, false};

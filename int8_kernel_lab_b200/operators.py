@@ -9,8 +9,9 @@ model runs between its convolutions (no reference counterpart).
 `launch_*` write into the caller's buffers and never allocate; the plain names
 allocate the result (and the group norm's workspace) on the launch's stream.
 Everything is asynchronous on `stream` (default: the current one), runs on the
-current CUDA device and may be captured into a graph.  Wrong arguments raise
-ValueError (types, sizes, devices) or Int8ConvError (the library's own checks).
+current CUDA device and may be captured into a graph.  Results carry no
+gradients.  Wrong arguments raise ValueError (types, sizes, devices) or
+Int8ConvError (the library's own checks).
 
 int8 matrices are rows of k bytes whose pitch is a multiple of 16 (the copies
 into shared memory move 16-byte units): the int8 results here come that way, as

@@ -1,6 +1,10 @@
 """The products, the row quantisation and the group norm against their plain
 64-bit forms (operators_reference.py), at the sizes, layouts and values where
 they can go wrong."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -388,6 +392,84 @@ def test_group_norm_in_place_and_deterministic(cuda):
         ws = torch.empty(m.group_norm_workspace_bytes(y, 8, y), dtype=torch.uint8, device="cuda")
         m.launch_group_norm(y, 8, y, activation="gelu", workspace=ws, workspace_bytes=ws.numel())
         assert torch.equal(y, want)
+
+
+def test_group_norm_channel_worth_nothing(cuda):
+    # A channel whose step is worth 0 is zero throughout, and still has a place
+    # in its group's statistics.
+    g = _gen(34)
+    x, scale = _norm_input(g, 2, 90, 40, torch.int32)
+    scale[[0, 13]] = 0
+    beta = torch.randn(40, generator=g, device="cuda")
+    y = m.group_norm(x, 5, beta=beta, scale=scale, activation="silu", dtype=torch.float32)
+    want, err = ref.norm(x, 5, None, beta, 1e-5, "silu", scale)
+    ref.check(y, want, err)
+
+
+def test_elements_past_two_to_the_31(cuda):
+    # Rows, pitches and results whose element offsets do not fit 32 bits.
+    g = _gen(35)
+    rows, n = 40000, 60000                       # 2.4e9 results
+    o = _operands(rows, n, 16, 36)
+    y = m.matmul(o["a"], o["b"], row_scale=o["row"], col_scale=o["col"], bias=o["bias"])
+    at = torch.tensor([0, 1, 35790, 35791, 35792, rows - 1], device="cuda")
+    want, err = ref.product(o["a"][at], o["b"], o["row"][at], o["col"], o["bias"])
+    ref.check(y[at], want, err)
+    q, scale = m.quantize_rows(y)
+    wq, wscale = ref.quantized(y[at])
+    assert torch.equal(q[at].cpu(), wq) and torch.equal(scale[at].cpu(), wscale)
+    back = m.matmul(q, q[:5], row_scale=scale, dtype=torch.float32)   # reads 2.4e9 bytes of a
+    want, err = ref.product(q[at], q[:5], scale[at])
+    ref.check(back[at], want, err)
+    index = torch.tensor([rows - 1, 35792], dtype=torch.int32, device="cuda")
+    assert torch.equal(m.quantize_rows(y, index)[0], q[index.long()])
+    del q, back
+    x = y.view(2, -1, 64)                        # 1.2e9 elements an image
+    z = m.group_norm(x, 1, activation="relu")
+    mean = x.float().mean((1, 2), keepdim=True, dtype=torch.float64)
+    var = torch.stack([(i.float() - c.float()).square().mean(dtype=torch.float64)
+                       for i, c in zip(x, mean)]).view(2, 1, 1)
+    for sl in (slice(0, 1000), slice(-1000, None)):
+        want = ((x[:, sl].double() - mean) / (var + 1e-5).sqrt()).clamp_min(0).cpu()
+        # 18.7e6 pixels over 296 CTAs of 64 threads a column: runs of 1000 additions.
+        ref.check(z[:, sl], want, want.abs() * 2000 * ref.U + 2000 * ref.U, "norm")
+
+
+def test_operators_from_two_streams_at_once(cuda):
+    args = [_block_inputs(40 + i) for i in range(2)]
+    want = [_block(*a) for a in args]
+    streams = [torch.cuda.Stream() for _ in args]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(_block(*args[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+    assert m.device_status() == _abi.OK
+
+
+def test_first_call_of_a_process_may_be_captured(cuda):
+    code = """
+import torch, int8_kernel_lab_b200 as m
+a = torch.ones(40, 64, dtype=torch.int8, device="cuda")
+x = torch.randn(40, 64, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    q, s = m.quantize_rows(x)
+    y = m.matmul(a, a, residual=None, dtype=torch.float32)
+    z = m.group_norm(x.view(2, 20, 64), 4)
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, torch.full((40, 40), 64.0, device="cuda")), y
+assert torch.equal(q, m.quantize_rows(x)[0]) and torch.equal(z, m.group_norm(x.view(2, 20, 64), 4))
+"""
+    root = Path(__file__).resolve().parent.parent
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                          timeout=120)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def _block(x, w1, c1, w2, c2, gamma, beta):
