@@ -13,7 +13,9 @@
 // quotient is a product with the rounded reciprocal, off by at most 3 half
 // steps (3 * 2^-24 * 127 = 2.3e-5): where it lies further than that from the
 // middle between two integers, both round alike; the few vectors with an
-// element nearer than 4e-5 are divided.
+// element nearer than 4e-5 are divided.  Now 89 us, 4.5 TB/s; what is left is
+// the latency from index to row to maximum, which 1536 threads an SM hide in
+// part.
 #include <cuda_runtime.h>
 
 #include "epilogue.cuh"
