@@ -12,16 +12,16 @@
 //                x again (from L2 while it fits there).
 //
 // A thread owns one vector of 8 channels and walks down the pixels: 16-byte
-// loads, a warp reads whole lines.  Sums are taken relative to the span's first
-// pixel (no cancellation for a large mean) in fp32, in the input's own units:
-// the channel scale is applied to the channel's mean and squares afterwards.
-// Threads, channels, CTAs and chunks are joined in a fixed order, so the result
-// does not depend on timing.
+// loads, a warp reads whole lines.  Sums are taken in fp32 about a shift that
+// follows the mean (span_stats), in the input's own units: the channel scale is
+// applied to the channel's mean and squares afterwards.  Threads, channels, CTAs
+// and chunks are joined as (mean, squared deviations) in a fixed order, so the
+// result does not depend on timing.
 //
-// Measured: 256 images of 3136 x 256 int32 to fp16 319 us, DRAM at 6.4 TB/s with x
+// Measured: 256 images of 3136 x 256 int32 to fp16 314 us, DRAM at 6.4 TB/s with x
 // read twice; 8 of 4096 x 320 bf16 to bf16 with silu 19 us, two kernels bound by
 // the latency of their loads and reductions (and, with silu, by the two special
-// functions of each element); one of 196 x 256 int32 6.4 us, where a launch alone
+// functions of each element); one of 196 x 256 int32 6.8 us, where a launch alone
 // takes 2.3.
 #include <cuda_runtime.h>
 #include <math.h>
@@ -206,8 +206,22 @@ __device__ __forceinline__ int rows_of(const NormArgs &a, int span) {
   return left <= 0 ? 0 : (left < a.span_pixels ? left : a.span_pixels);
 }
 
+// Batches of a run: a thread adds the squares of this many batches before it adds
+// the run's sum to the runs' before it.
+constexpr int kRun = 16;
+
 // (mean, squared deviations) of every group over pixels [0, rows) of x, this
 // CTA's span, into part[].  `mine`: the parameters of channel threadIdx.x.
+//
+// A thread sums d = x - shift and d^2 of its own pixels, the shift its first
+// pixel.  After 1, 2, 4 and so on up to kRun batches, and after every run from
+// then on, the shift moves to the mean so far, the sums with it:
+//   e = s1 / n,  s2 <- s2 - e (2 s1 - n e),  s1 <- s1 - n e,  shift <- shift + e
+// No step cancels, wherever an outlier lies: the shift is one of the values or
+// the mean of at least half of them, so the squares about it are at most n times
+// the squared deviations in the first batch (n <= 8), and later at most twice.
+// The longest chain of additions of squares is kRun batches, then the runs.  A thread's squares of finished runs lie in its `cell`, which
+// is free until the sums are joined.
 template <int DT, int VEC>
 __device__ __forceinline__ void span_stats(const NormArgs &a, const typename Elem<DT>::type *x,
                                            int rows, uint8_t *area, float *cell,
@@ -220,16 +234,15 @@ __device__ __forceinline__ void span_stats(const NormArgs &a, const typename Ele
   for (int col0 = 0; col0 < cols; col0 += kThreads) {
     const Columns k(cols, col0);
     const bool active = k.part < k.lanes;
+    const int wide = k.width * VEC, c0 = col0 * VEC;
+    float *own = cell + k.part * wide + k.col * VEC;   // this thread's place (active threads)
+    const int pixels = active && k.part < rows ? (rows - k.part - 1) / k.lanes + 1 : 0;
     float x0[VEC], s1[VEC], s2[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) x0[j] = s1[j] = s2[j] = 0.f;
-    if (active && rows > 0) {
-      const T *at = x + (col0 + k.col) * VEC;
-      Raw<DT, VEC> shift;
-      shift.load(at);
-      at += k.part * a.ldx;
+    if (pixels > 0) {
+      const T *at = x + (col0 + k.col) * VEC + k.part * a.ldx;
       const int64_t step = k.lanes * a.ldx;
-      int left = k.part < rows ? (rows - k.part - 1) / k.lanes + 1 : 0;   // this thread's pixels
       auto add = [&](const Raw<DT, VEC> &r) {
         if constexpr (VEC == 1) {
           const float d = r.get(0) - x0[0];
@@ -244,16 +257,30 @@ __device__ __forceinline__ void span_stats(const NormArgs &a, const typename Ele
           }
         }
       };
-      bool first = true;
+      // The sums of n pixels move to their mean (to any value near it: the sums
+      // are exact about the shift, whatever it is).
+      auto center = [&](float n) {
+        const float inv = rcp_approx(n);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float to = fmaf(s1[j], inv, x0[j]);
+          const float e = to - x0[j];
+          const float rest = fmaf(-n, e, s1[j]);
+          s2[j] = fmaf(-e, s1[j] + rest, s2[j]);
+          s1[j] = rest;
+          x0[j] = to;
+        }
+      };
+      int left = pixels, done = 0, until = 1;   // batches done, and when to center next
+      int centered = 1;                         // pixels of the sums when last centered
 #pragma unroll 1
       for (; left >= kBatch; left -= kBatch) {
         Raw<DT, VEC> r[kBatch];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u, at += step) r[u].load(at);
-        if (first) {   // the shift was on its way together with the first batch
+        if (done == 0) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) x0[j] = shift.get(j);
-          first = false;
+          for (int j = 0; j < VEC; ++j) x0[j] = r[0].get(j);
         }
         if constexpr (VEC > 1) {
           if (kept > 0) {
@@ -265,55 +292,83 @@ __device__ __forceinline__ void span_stats(const NormArgs &a, const typename Ele
         }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) add(r[u]);
-      }
-      if (first) {
+        if (++done == until) {
+          if (done > kRun) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) x0[j] = shift.get(j);
+            for (int j = 0; j < VEC; ++j) s2[j] += own[j];
+          }
+          center(static_cast<float>(done * kBatch));
+          centered = done * kBatch;
+          if (done >= kRun) {
+            put_vec<VEC>(own, s2);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) s2[j] = 0.f;
+          }
+          until += done < kRun ? done : kRun;
+        }
       }
 #pragma unroll 1
       for (; left > 0; --left, at += step) {
         Raw<DT, VEC> r;
         r.load(at);
+        if (left == pixels) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) x0[j] = r.get(j);
+        }
         add(r);
       }
+      if (done >= kRun) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s2[j] += own[j];
+      }
+      // Now the mean and the squared deviations.
+      if (pixels > centered) center(static_cast<float>(pixels));
     }
-    // The sums of a column's threads, first all of one kind, then of the other
-    // through the same memory: cell[thread of the column][channel].
-    const int wide = k.width * VEC, c0 = col0 * VEC;
-    const float inv = 1.f / static_cast<float>(rows > 0 ? rows : 1);
+    // The threads of a column join: first the means, relative to the first
+    // thread's, then the squared deviations about the mean of all.  The first
+    // `more` threads hold one pixel more than the others.
+    const int each = rows / k.lanes, more = rows - each * k.lanes;
     auto gather = [&](const float (&v)[VEC]) {
-      if (active) put_vec<VEC>(cell + k.part * wide + k.col * VEC, v);
+      if (active) put_vec<VEC>(own, v);
       __syncthreads();
     };
-    auto total = [&](int i) {
-      float t = 0.f;
-#pragma unroll 4
-      for (int q = 0; q < k.lanes; ++q) t += cell[q * wide + i];
-      return t;
-    };
-    if (k.part == 0) {
-      // The threads without a pixel hold no shift; the first has one.
-      if (rows > 0) {
-        put_vec<VEC>(ch.m + c0 + k.col * VEC, x0);
-      } else {
+    gather(x0);
+    const float inv = 1.f / static_cast<float>(rows > 0 ? rows : 1);
+#pragma unroll 1
+    for (int i = threadIdx.x; i < wide; i += kThreads) {
+      const float ref = cell[i];
+      float all = 0.f, head = 0.f;
+#pragma unroll 8
+      for (int q = 0; q < k.lanes; ++q) {
+        const float d = cell[q * wide + i] - ref;
+        all += d;
+        if (q < more) head += d;
+      }
+      const float sum = fmaf(static_cast<float>(each), all, head);
+      ch.m[c0 + i] = fmaf(sum, inv, ref);
+    }
+    __syncthreads();
+    if (pixels > 0) {
+      const float n = static_cast<float>(pixels);
+      float mean[VEC];
+      get_vec<VEC>(ch.m + c0 + k.col * VEC, mean);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) ch.m[c0 + k.col * VEC + j] = 0.f;
+      for (int j = 0; j < VEC; ++j) {
+        const float d = x0[j] - mean[j];
+        // s2 is not below zero but for a rounding; NaN stays NaN.
+        s2[j] = fmaf(d * n, d, s2[j] < 0.f ? 0.f : s2[j]);
       }
     }
-    gather(s1);
-#pragma unroll 1
-    for (int i = threadIdx.x; i < wide; i += kThreads) ch.w[c0 + i] = total(i);
-    __syncthreads();
     gather(s2);
 #pragma unroll 1
     for (int i = threadIdx.x; i < wide; i += kThreads) {
       const int c = c0 + i;
       const float s = c == static_cast<int>(threadIdx.x) ? mine.scale : Params(a, c).scale;
-      const float sum = ch.w[c];
-      const float d = sum * inv;
-      const float sq = total(i) - sum * d;     // not below zero; NaN stays NaN
-      ch.m[c] = (ch.m[c] + d) * s;
-      ch.w[c] = (sq < 0.f ? 0.f : sq) * s * s;
+      float sq = 0.f;
+#pragma unroll 8
+      for (int q = 0; q < k.lanes; ++q) sq += cell[q * wide + i];
+      ch.m[c] *= s;
+      ch.w[c] = sq * s * s;
     }
     __syncthreads();
   }

@@ -1,0 +1,107 @@
+"""The group norm's statistics where a few positions lie far from the others:
+the corner of a zero-padded image, a first token with massive activations."""
+import pytest
+import torch
+
+import int8_kernel_lab_b200 as m
+from operators_reference import HALF, U
+
+pytestmark = pytest.mark.gpu
+
+
+def _exact(x, groups, scale=None):
+    """(normalised values, mean / deviation) of one image [p, c] in 64 bits, on the GPU."""
+    v = x.double()
+    if scale is not None:
+        v = v * scale.double()
+    p, c = v.shape
+    v = v.view(p, groups, c // groups)
+    var, mean = torch.var_mean(v, dim=(0, 2), unbiased=False, keepdim=True)
+    rstd = 1 / (var + 1e-5).sqrt()
+    return ((v - mean) * rstd).view(p, c), (mean.abs() * rstd).expand_as(v).reshape(p, c), \
+        (v.abs() * rstd).reshape(p, c)
+
+
+def _tolerance(z, mean, size, p, c, vec):
+    """Half an fp32 step is u.  A run of a thread is at most 128 positions.
+
+    Variance: the squares added are never more than twice what they come to (8
+    times in a first batch of 8), so its relative error is the additions' chain:
+    2 * (128 + runs) + 64 of a thread, up to `lanes` threads of a column, 32
+    steps over channels and CTAs.  Half of it reaches 1 / deviation.
+    Mean, in deviations: a run's sum starts near zero, so 128 steps of the
+    values' mean distance (below 1.5 deviations, 200 in all); the threads' means
+    relative to the first one's, which may be sqrt(lanes) deviations away, over
+    `lanes` steps; the mean's own rounding, and its use in the input's units.
+    Each value times its scale, and the formula's own four roundings, come on top."""
+    lanes = 512 // min(512, c // 8 if vec else c)
+    chain = 2 * (128 + p / (32 * lanes) + 1) + 64 + lanes + 32
+    return U * (z.abs() * (chain / 2 + 4) + 200 + lanes ** 1.5 + 4 * mean + 4 * size)
+
+
+def _check(x, groups, scale=None):
+    n, p, c = x.shape
+    y = m.group_norm(x, groups, scale=scale, dtype=torch.float32)
+    for i in range(n):
+        z, mean, size = _exact(x[i], groups, scale)
+        off = (y[i].double() - z).abs()
+        tol = _tolerance(z, mean, size, p, c, c % 8 == 0)
+        worst = float((off / tol).max())
+        assert worst <= 1, f"image {i}: {worst:.3g} of the tolerance"
+    assert m.device_status() == 0
+
+
+@pytest.mark.parametrize("far", [100.0, 10000.0, "padding"])
+@pytest.mark.parametrize("n,p,c,groups", [
+    (256, 3136, 256, 32),     # a CTA for each image
+    (256, 4096, 260, 10),     # channel by channel, one thread down each
+    (256, 4096, 258, 258),
+    (40, 3000, 128, 4),       # clusters
+    (4, 16384, 64, 8),        # chunks, two kernels
+    (1, 200000, 8, 2),
+    (3, 5, 64, 8),            # less than a batch for each thread
+    (300, 70, 4096, 32),      # one thread down each column of 8 channels
+], ids=str)
+def test_first_position_far_from_the_others(cuda, n, p, c, groups, far):
+    g = torch.Generator(device="cuda").manual_seed(60)
+    x = torch.randn(n, p, c, generator=g, device="cuda")
+    if far == "padding":
+        x += 1000
+        x[:, 0] = 0
+    else:
+        x[:, 0] = far
+    _check(x, groups)
+
+
+@pytest.mark.parametrize("at", [1, 37, 1500, 2999])
+def test_far_position_anywhere(cuda, at):
+    x = torch.randn(20, 3000, 72, generator=torch.Generator(device="cuda").manual_seed(61),
+                    device="cuda")
+    x[:, at] = -3000.0
+    _check(x, 9)
+    _check(x[..., :70].contiguous(), 7)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.int32], ids=str)
+@pytest.mark.parametrize("n,p,c,groups", [(256, 3136, 128, 32), (8, 4096, 320, 32)], ids=str)
+def test_far_first_position_of_other_types(cuda, dtype, n, p, c, groups):
+    g = torch.Generator(device="cuda").manual_seed(62)
+    x = torch.randn(n, p, c, generator=g, device="cuda") + 3
+    x[:, 0] = 2000
+    scale = None
+    if dtype == torch.int32:
+        scale = (torch.rand(c, generator=g, device="cuda") + 0.5) / 2000
+        x = x * 2000
+    _check(x.to(dtype), groups, scale)
+
+
+def test_results_of_16_bits_are_rounded_once(cuda):
+    x = torch.randn(256, 1000, 64, generator=torch.Generator(device="cuda").manual_seed(63),
+                    device="cuda")
+    x[:, 0] = 500
+    y = m.group_norm(x, 8, dtype=torch.float16)
+    for i in range(0, 256, 50):
+        z, mean, size = _exact(x[i], 8)
+        tol = _tolerance(z, mean, size, 1000, 64, True)
+        tol = tol + (z.abs() + tol) * HALF[torch.float16] + 2.0 ** -25
+        assert bool(((y[i].double() - z).abs() <= tol).all())
