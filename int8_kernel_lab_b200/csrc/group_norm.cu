@@ -13,10 +13,12 @@
 //
 // A thread owns one vector of 8 channels and walks down the pixels: 16-byte
 // loads, a warp reads whole lines.  Sums are taken in fp32 about a shift that
-// follows the mean (span_stats), in the input's own units: the channel scale is
-// applied to the channel's mean and squares afterwards.  Threads, channels, CTAs
-// and chunks are joined as (mean, squared deviations) in a fixed order, so the
-// result does not depend on timing.
+// follows the mean (span_stats), of float inputs with a scale as x * scale -
+// shift, so that x may have any size that the scale makes ordinary.  int32 inputs
+// are summed as they are (no square of theirs leaves fp32's range), and the scale
+// is applied to the channel's mean and squares.  Threads, channels, CTAs and
+// chunks are joined as (mean, squared deviations) in a fixed order, so the result
+// does not depend on timing.
 //
 // Measured: 256 images of 3136 x 256 int32 to fp16 314 us, DRAM at 6.4 TB/s with x
 // read twice; 8 of 4096 x 320 bf16 to bf16 with silu 19 us, two kernels bound by
@@ -210,8 +212,8 @@ __device__ __forceinline__ int rows_of(const NormArgs &a, int span) {
 // the run's sum to the runs' before it.
 constexpr int kRun = 16;
 
-// (mean, squared deviations) of every group over pixels [0, rows) of x, this
-// CTA's span, into part[].  `mine`: the parameters of channel threadIdx.x.
+// (mean, squared deviations) of every channel over pixels [0, rows) of x, this
+// CTA's span, into ch.m and ch.w.  `mine`: the parameters of channel threadIdx.x.
 //
 // A thread sums d = x - shift and d^2 of its own pixels, the shift its first
 // pixel.  After 1, 2, 4 and so on up to kRun batches, and after every run from
@@ -220,12 +222,13 @@ constexpr int kRun = 16;
 // No step cancels, wherever an outlier lies: the shift is one of the values or
 // the mean of at least half of them, so the squares about it are at most n times
 // the squared deviations in the first batch (n <= 8), and later at most twice.
-// The longest chain of additions of squares is kRun batches, then the runs.  A thread's squares of finished runs lie in its `cell`, which
-// is free until the sums are joined.
-template <int DT, int VEC>
-__device__ __forceinline__ void span_stats(const NormArgs &a, const typename Elem<DT>::type *x,
-                                           int rows, uint8_t *area, float *cell,
-                                           const Channels &ch, const Params &mine, float2 *part) {
+// The longest chain of additions of squares is kRun batches, then the runs.  A
+// thread's squares of finished runs lie in its `cell`, which is free until the
+// sums are joined.  SCALED: each value times its channel's scale.
+template <int DT, int VEC, bool SCALED>
+__device__ __forceinline__ void span_sums(const NormArgs &a, const typename Elem<DT>::type *x,
+                                          int rows, uint8_t *area, float *cell,
+                                          const Channels &ch, const Params &mine) {
   using T = typename Elem<DT>::type;
   constexpr int kBatch = batch<DT, VEC>();
   const int cols = a.channels / VEC;
@@ -241,20 +244,37 @@ __device__ __forceinline__ void span_stats(const NormArgs &a, const typename Ele
 #pragma unroll
     for (int j = 0; j < VEC; ++j) x0[j] = s1[j] = s2[j] = 0.f;
     if (pixels > 0) {
+      [[maybe_unused]] float by[VEC];
+      if constexpr (SCALED) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) by[j] = __ldg(a.scale + c0 + k.col * VEC + j);
+      }
       const T *at = x + (col0 + k.col) * VEC + k.part * a.ldx;
       const int64_t step = k.lanes * a.ldx;
       auto add = [&](const Raw<DT, VEC> &r) {
         if constexpr (VEC == 1) {
-          const float d = r.get(0) - x0[0];
+          const float d = SCALED ? fmaf(r.get(0), by[0], -x0[0]) : r.get(0) - x0[0];
           s1[0] += d;
           s2[0] = fmaf(d, d, s2[0]);
         } else {
 #pragma unroll
           for (int j = 0; j < VEC; j += 2) {
-            const uint64_t d = f2_add(r.pair(j), f2_pack(-x0[j], -x0[j + 1]));
+            const uint64_t minus = f2_pack(-x0[j], -x0[j + 1]);
+            uint64_t d;
+            if constexpr (SCALED)
+              d = f2_fma(r.pair(j), f2_pack(by[j], by[j + 1]), minus);
+            else
+              d = f2_add(r.pair(j), minus);
             f2_unpack(f2_add(f2_pack(s1[j], s1[j + 1]), d), s1[j], s1[j + 1]);
             f2_unpack(f2_fma(d, d, f2_pack(s2[j], s2[j + 1])), s2[j], s2[j + 1]);
           }
+        }
+      };
+      auto start = [&](const Raw<DT, VEC> &r) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          x0[j] = r.get(j);
+          if constexpr (SCALED) x0[j] *= by[j];
         }
       };
       // The sums of n pixels move to their mean (to any value near it: the sums
@@ -278,10 +298,7 @@ __device__ __forceinline__ void span_stats(const NormArgs &a, const typename Ele
         Raw<DT, VEC> r[kBatch];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u, at += step) r[u].load(at);
-        if (done == 0) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) x0[j] = r[0].get(j);
-        }
+        if (done == 0) start(r[0]);
         if constexpr (VEC > 1) {
           if (kept > 0) {
 #pragma unroll
@@ -311,18 +328,19 @@ __device__ __forceinline__ void span_stats(const NormArgs &a, const typename Ele
       for (; left > 0; --left, at += step) {
         Raw<DT, VEC> r;
         r.load(at);
-        if (left == pixels) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) x0[j] = r.get(j);
-        }
+        if (left == pixels) start(r);
         add(r);
       }
       if (done >= kRun) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) s2[j] += own[j];
       }
-      // Now the mean and the squared deviations.
+      // Now the mean, and the squares about it: less those of what its rounding
+      // left, the squared deviations.
       if (pixels > centered) center(static_cast<float>(pixels));
+      const float inv = rcp_approx(static_cast<float>(pixels));
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s2[j] = fmaf(-s1[j] * inv, s1[j], s2[j]);
     }
     // The threads of a column join: first the means, relative to the first
     // thread's, then the squared deviations about the mean of all.  The first
@@ -363,15 +381,30 @@ __device__ __forceinline__ void span_stats(const NormArgs &a, const typename Ele
 #pragma unroll 1
     for (int i = threadIdx.x; i < wide; i += kThreads) {
       const int c = c0 + i;
-      const float s = c == static_cast<int>(threadIdx.x) ? mine.scale : Params(a, c).scale;
       float sq = 0.f;
 #pragma unroll 8
       for (int q = 0; q < k.lanes; ++q) sq += cell[q * wide + i];
-      ch.m[c] *= s;
-      ch.w[c] = sq * s * s;
+      if constexpr (SCALED) {
+        ch.w[c] = sq;
+      } else {
+        const float s = c == static_cast<int>(threadIdx.x) ? mine.scale : Params(a, c).scale;
+        ch.m[c] *= s;
+        ch.w[c] = sq * s * s;
+      }
     }
     __syncthreads();
   }
+}
+
+// The same of every group, into part[].
+template <int DT, int VEC>
+__device__ __forceinline__ void span_stats(const NormArgs &a, const typename Elem<DT>::type *x,
+                                           int rows, uint8_t *area, float *cell,
+                                           const Channels &ch, const Params &mine, float2 *part) {
+  if (DT != INT8CONV_INT32 && a.scale != nullptr)
+    span_sums<DT, VEC, DT != INT8CONV_INT32>(a, x, rows, area, cell, ch, mine);
+  else
+    span_sums<DT, VEC, false>(a, x, rows, area, cell, ch, mine);
   // Channels of a group all hold `rows` values: the mean of means (relative to
   // the first, so that a large mean costs no bits), and the squares plus `rows`
   // times the means' squared deviations.  2 to 32 lanes share a group.

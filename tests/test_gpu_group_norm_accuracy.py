@@ -105,3 +105,25 @@ def test_results_of_16_bits_are_rounded_once(cuda):
         tol = _tolerance(z, mean, size, 1000, 64, True)
         tol = tol + (z.abs() + tol) * HALF[torch.float16] + 2.0 ** -25
         assert bool(((y[i].double() - z).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("n,p,c,groups", [(2, 90, 64, 8), (3, 4000, 40, 5), (1, 700, 30, 3)], ids=str)
+@pytest.mark.parametrize("size", [1e-30, 1e-22, 1e22, 1e30])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_scale_makes_small_and_large_inputs_ordinary(cuda, dtype, size, n, p, c, groups):
+    # The squares of x leave fp32's range, those of x * scale do not.
+    g = torch.Generator(device="cuda").manual_seed(64)
+    x = (torch.randn(n, p, c, generator=g, device="cuda") + 2).to(dtype)
+    scale = torch.rand(c, generator=g, device="cuda") + 0.5
+    scale[::3] /= size
+    x[..., ::3] = (x[..., ::3].float() * size).to(dtype)
+    _check(x, groups, scale)
+
+
+def test_constant_channels_under_a_scale(cuda):
+    # x * scale is rounded alike everywhere: the deviations are zero.
+    x = torch.full((2, 500, 32), 12345.0, device="cuda")
+    scale = torch.full((32,), 0.37, device="cuda")
+    y = m.group_norm(x, 4, scale=scale, eps=1e-5)
+    # The mean and its use in x's units are off by 2 u of the value, over sqrt(eps).
+    assert float(y.abs().max()) <= 4 * U * 12345 * 0.37 / 1e-5 ** 0.5
