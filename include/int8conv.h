@@ -280,7 +280,8 @@ int8conv_status int8conv_launch_quantize_rows(int64_t m, int64_t k, int32_t x_dt
  * pixels * ldy.  channels % groups == 0, channels <= INT8CONV_MAX_NORM_CHANNELS,
  * groups <= INT8CONV_MAX_NORM_GROUPS.
  * y may be x itself where types and pitches are equal.  Statistics are held in
- * fp32 as (mean, squared deviations) pairs, joined in a fixed order. */
+ * fp32 as (mean, squared deviations) pairs, joined in a fixed order; v, its
+ * square and scale / deviation have to stay within fp32's range, x need not. */
 typedef struct int8conv_group_norm {
   int64_t n, pixels;
   int32_t channels, groups;

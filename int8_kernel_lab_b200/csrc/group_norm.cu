@@ -445,12 +445,15 @@ __device__ __forceinline__ void channel_constants(const NormArgs &a, const float
     const Params p = c == static_cast<int>(threadIdx.x) ? mine : Params(a, c);
     const float2 t = stat[c / a.per_group];
     const float w = t.y * p.gamma;
-    if (p.scale == 0.f) {     // a channel that is zero throughout
+    const float m = p.scale == 1.f ? t.x : t.x / p.scale;
+    if (!(fabsf(m) <= 1e37f)) {
+      // A channel that is worth next to nothing beside the group's mean, or
+      // nothing: the mean goes into the offset.
       ch.m[c] = 0.f;
-      ch.w[c] = 0.f;
+      ch.w[c] = w * p.scale;
       ch.b[c] = fmaf(-t.x, w, p.beta);
     } else {
-      ch.m[c] = p.scale == 1.f ? t.x : t.x / p.scale;
+      ch.m[c] = m;
       ch.w[c] = w * p.scale;
       ch.b[c] = p.beta;
     }

@@ -127,3 +127,14 @@ def test_constant_channels_under_a_scale(cuda):
     y = m.group_norm(x, 4, scale=scale, eps=1e-5)
     # The mean and its use in x's units are off by 2 u of the value, over sqrt(eps).
     assert float(y.abs().max()) <= 4 * U * 12345 * 0.37 / 1e-5 ** 0.5
+
+
+@pytest.mark.parametrize("n,p,c,groups", [(2, 90, 64, 8), (3, 4000, 40, 5), (1, 700, 30, 3)], ids=str)
+@pytest.mark.parametrize("small", [1e-30, -1e-32, 0.0])
+def test_channel_far_smaller_than_its_group(cuda, small, n, p, c, groups):
+    # The group's mean in the units of such a channel leaves fp32's range.
+    g = torch.Generator(device="cuda").manual_seed(65)
+    x = torch.randn(n, p, c, generator=g, device="cuda") * 1e8 + 1e9
+    scale = torch.rand(c, generator=g, device="cuda") + 0.5
+    scale[1::4] = small
+    _check(x, groups, scale)
