@@ -63,19 +63,49 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // Activations in fp32, two values at a time: the products and sums as pairs.
 //   silu       v / (1 + 2^(-v log2 e))
 //   gelu_tanh  (1 + tanh u) / 2 = 1 / (1 + exp(-2u)): v / (1 + 2^(-v (p + q v^2)))
-//   gelu       v Phi(v) with Phi from the complementary error function of
-//              Abramowitz and Stegun 7.1.26: for z = |v| / sqrt 2, t = 1 / (1 + p z),
-//              erfc(z) = t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-z^2) + e, |e| <= 1.5e-7;
-//              Phi = erfc / 2 below zero, 1 - erfc / 2 above.
-// Errors stay below 2^-19 |v|: the exponent's argument is rounded at most
-// three times (|v| < 10: 14.4 * 3 * 2^-24, times a quotient below one), the
-// exponential and the quotient add 2^-22 each.  Large negative v: the power
-// overflows to infinity, its reciprocal is 0, the result -0; NaN stays NaN.
-template <int ACT>
+//   gelu       v Phi(v): with z = |v| / sqrt 2, Phi = erfc(z) / 2 below zero and
+//              1 - erfc(z) / 2 above; erfc(z) / 2 = exp(-z^2) t P(t), t = 1 / (1 + 0.33 z).
+//              P is the polynomial of degree 7 whose largest relative error over
+//              0 <= z <= 9.5 is least (8.2e-8; fitted to exp(z^2) erfc(z) by
+//              least squares with Lawson's weights).
+// FULL, for fp32 results: silu with the rest of its exponent, gelu for |v| <= 1 as
+// v / 2 + v^2 R(v^2), R the polynomial of degree 4 fitted to (Phi(v) - 1/2) / v in
+// the same way (2.9e-8 of the result); gelu_tanh is as near as fp32 allows anyway.
+//
+// Largest errors relative to the result, in u = 2^-24 (each exponential has
+// 4 u, each reciprocal 2 u, each product or sum 1 u; an exponent x rounded k
+// times adds 0.69 k |x| u to 2^x), measured over 4 million values, beside
+// those of torch's fp32 forms:
+//                         v >= -0.5   -2..-0.5   -6..-2
+//   silu                     4.0         4.0       8.3
+//   silu, FULL               3.5         4.0       4.0
+//   gelu_tanh                3.6         7.5      54        (exponents to 36, three roundings)
+//   gelu                    10.4         9.6      32       (exponents to 26, two roundings)
+//   gelu, FULL               2.2         9.6      32
+//   silu, torch              3.1         3.1       3.4
+//   gelu_tanh, torch         2.9        18        all of it
+//   gelu, torch              2.7        20        all of it
+// Large negative v: the power overflows to infinity, its reciprocal is 0, the
+// result -0; NaN stays NaN.
+template <int ACT, bool FULL = false>
 __device__ __forceinline__ void activate2(float &a, float &b) {
   if constexpr (ACT == INT8CONV_ACT_RELU) {
     a = a < 0.f ? 0.f : a;
     b = b < 0.f ? 0.f : b;
+  } else if constexpr (ACT == INT8CONV_ACT_SILU && FULL) {
+    // The power of the rounded exponent x, times 1 - ln 2 (what x lacks): d from
+    // the rounding of the product, v * 1.9e-8 from that of log2 e.
+    const uint64_t v = f2_pack(fminf(a, 100.f), fminf(b, 100.f));
+    const uint64_t x = f2_mul(v, f2_pack(-1.44269502f, -1.44269502f));
+    const uint64_t d = f2_fma(v, f2_pack(1.44269502f, 1.44269502f), x);
+    const uint64_t t = f2_fma(v, f2_pack(1.92596299e-8f, 1.92596299e-8f), d);
+    float e0, e1;
+    f2_unpack(x, e0, e1);
+    const uint64_t e = f2_pack(fminf(exp2_approx(e0), 3e38f), fminf(exp2_approx(e1), 3e38f));
+    const uint64_t s = f2_fma(f2_mul(e, t), f2_pack(-0.69314718f, -0.69314718f), e);
+    f2_unpack(f2_add(s, f2_pack(1.f, 1.f)), e0, e1);
+    a *= rcp_approx(e0);
+    b *= rcp_approx(e1);
   } else if constexpr (ACT == INT8CONV_ACT_SILU || ACT == INT8CONV_ACT_GELU_TANH) {
     const uint64_t v = f2_pack(a, b);
     uint64_t x;
@@ -93,29 +123,48 @@ __device__ __forceinline__ void activate2(float &a, float &b) {
     f2_unpack(x, e0, e1);
     f2_unpack(f2_mul(v, f2_pack(rcp_approx(e0), rcp_approx(e1))), a, b);
   } else if constexpr (ACT == INT8CONV_ACT_GELU) {
-    const uint64_t z = f2_mul(f2_pack(fabsf(a), fabsf(b)),
-                              f2_pack(0.70710678118654752f, 0.70710678118654752f));
+    // 1 + 0.33 z
     float e0, e1;
-    f2_unpack(f2_fma(z, f2_pack(0.3275911f, 0.3275911f), f2_pack(1.f, 1.f)), e0, e1);
+    f2_unpack(f2_fma(f2_pack(fabsf(a), fabsf(b)), f2_pack(0.23334524f, 0.23334524f),
+                     f2_pack(1.f, 1.f)),
+              e0, e1);
     const uint64_t t = f2_pack(rcp_approx(e0), rcp_approx(e1));
-    // The coefficients are halved: half of erfc.
-    uint64_t h = f2_pack(0.5307027145f, 0.5307027145f);
-    h = f2_fma(h, t, f2_pack(-0.7265760135f, -0.7265760135f));
-    h = f2_fma(h, t, f2_pack(0.7107068705f, 0.7107068705f));
-    h = f2_fma(h, t, f2_pack(-0.142248368f, -0.142248368f));
-    h = f2_fma(h, t, f2_pack(0.127414796f, 0.127414796f));
-    f2_unpack(f2_mul(f2_mul(z, z), f2_pack(-1.4426950408889634f, -1.4426950408889634f)), e0, e1);
+    uint64_t h = f2_pack(-0.0679643707f, -0.0679643707f);
+    h = f2_fma(h, t, f2_pack(0.231343964f, 0.231343964f));
+    h = f2_fma(h, t, f2_pack(-0.177719227f, -0.177719227f));
+    h = f2_fma(h, t, f2_pack(0.206270591f, 0.206270591f));
+    h = f2_fma(h, t, f2_pack(0.0225054312f, 0.0225054312f));
+    h = f2_fma(h, t, f2_pack(0.100961884f, 0.100961884f));
+    h = f2_fma(h, t, f2_pack(0.0914186293f, 0.0914186293f));
+    h = f2_fma(h, t, f2_pack(0.0931830583f, 0.0931830583f));
+    // 2^(-v^2 log2 e / 2)
+    const uint64_t v = f2_pack(a, b);
+    f2_unpack(f2_mul(f2_mul(v, v), f2_pack(-0.72134752044448170f, -0.72134752044448170f)), e0, e1);
     h = f2_mul(f2_mul(h, t), f2_pack(exp2_approx(e0), exp2_approx(e1)));
     f2_unpack(h, e0, e1);
-    a *= a < 0.f ? e0 : 1.f - e0;
-    b *= b < 0.f ? e1 : 1.f - e1;
+    if constexpr (FULL) {
+      const uint64_t w = f2_mul(v, v);
+      uint64_t r = f2_pack(9.15124104e-5f, 9.15124104e-5f);
+      r = f2_fma(r, w, f2_pack(-0.00116311492f, -0.00116311492f));
+      r = f2_fma(r, w, f2_pack(0.00996239664f, 0.00996239664f));
+      r = f2_fma(r, w, f2_pack(-0.0664881962f, -0.0664881962f));
+      r = f2_fma(r, w, f2_pack(0.398942153f, 0.398942153f));
+      r = f2_fma(r, w, f2_mul(v, f2_pack(0.5f, 0.5f)));
+      float n0, n1;
+      f2_unpack(r, n0, n1);
+      a = fabsf(a) <= 1.f ? n0 : a * (a < 0.f ? e0 : 1.f - e0);
+      b = fabsf(b) <= 1.f ? n1 : b * (b < 0.f ? e1 : 1.f - e1);
+    } else {
+      a *= a < 0.f ? e0 : 1.f - e0;
+      b *= b < 0.f ? e1 : 1.f - e1;
+    }
   }
 }
 
-template <int ACT>
+template <int ACT, bool FULL = false>
 __device__ __forceinline__ float activate(float v) {
   float unused = 0.f;
-  activate2<ACT>(v, unused);
+  activate2<ACT, FULL>(v, unused);
   return v;
 }
 

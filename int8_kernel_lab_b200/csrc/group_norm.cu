@@ -487,14 +487,14 @@ __device__ __forceinline__ void apply_span(const NormArgs &a, const typename Ele
     auto finish = [&](const Raw<DT, VEC> &r) {
       float f[VEC];
       if constexpr (VEC == 1) {
-        f[0] = activate<ACT>(fmaf(r.get(0) - m[0], w[0], b[0]));
+        f[0] = activate<ACT, OUT == INT8CONV_FP32>(fmaf(r.get(0) - m[0], w[0], b[0]));
         if constexpr (OUT == INT8CONV_INT8) f[0] *= a.inv_out_scale;
       } else {
 #pragma unroll
         for (int j = 0; j < VEC; j += 2) {
           const uint64_t d = f2_add(r.pair(j), f2_pack(-m[j], -m[j + 1]));
           f2_unpack(f2_fma(d, f2_pack(w[j], w[j + 1]), f2_pack(b[j], b[j + 1])), f[j], f[j + 1]);
-          activate2<ACT>(f[j], f[j + 1]);
+          activate2<ACT, OUT == INT8CONV_FP32>(f[j], f[j + 1]);
           if constexpr (OUT == INT8CONV_INT8)
             f2_unpack(f2_mul(f2_pack(f[j], f[j + 1]), f2_pack(a.inv_out_scale, a.inv_out_scale)),
                       f[j], f[j + 1]);

@@ -197,7 +197,7 @@ __device__ __forceinline__ void commit_mma(uint64_t *bar) {
 
 // scale, bias and activation of one 32-column block of a thread's row;
 // `table`: the block's columns in pairs, (scale, scale, bias, bias).
-template <int ACT>
+template <int ACT, int OUT>
 __device__ __forceinline__ void finish_block(uint32_t (&v)[32], float rs, const float4 *table) {
   const uint64_t row = f2_pack(rs, rs);
 #pragma unroll
@@ -207,7 +207,7 @@ __device__ __forceinline__ void finish_block(uint32_t (&v)[32], float rs, const 
                                static_cast<float>(static_cast<int32_t>(v[2 * j + 1])));
     float a, b;
     f2_unpack(f2_fma(f2_mul(x, f2_pack(t.x, t.y)), row, f2_pack(t.z, t.w)), a, b);
-    activate2<ACT>(a, b);
+    activate2<ACT, OUT == INT8CONV_FP32>(a, b);
     v[2 * j] = __float_as_uint(a);
     v[2 * j + 1] = __float_as_uint(b);
   }
@@ -666,19 +666,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float4 *tb = reinterpret_cast<const float4 *>(table) + i * 16;
           switch (g.activation) {
             case INT8CONV_ACT_RELU:
-              finish_block<INT8CONV_ACT_RELU>(v, rs, tb);
+              finish_block<INT8CONV_ACT_RELU, OUT>(v, rs, tb);
               break;
             case INT8CONV_ACT_GELU:
-              finish_block<INT8CONV_ACT_GELU>(v, rs, tb);
+              finish_block<INT8CONV_ACT_GELU, OUT>(v, rs, tb);
               break;
             case INT8CONV_ACT_GELU_TANH:
-              finish_block<INT8CONV_ACT_GELU_TANH>(v, rs, tb);
+              finish_block<INT8CONV_ACT_GELU_TANH, OUT>(v, rs, tb);
               break;
             case INT8CONV_ACT_SILU:
-              finish_block<INT8CONV_ACT_SILU>(v, rs, tb);
+              finish_block<INT8CONV_ACT_SILU, OUT>(v, rs, tb);
               break;
             default:
-              finish_block<INT8CONV_ACT_NONE>(v, rs, tb);
+              finish_block<INT8CONV_ACT_NONE, OUT>(v, rs, tb);
           }
           if constexpr (kResidual) {
             if (res != nullptr) {
@@ -748,16 +748,17 @@ __device__ __forceinline__ int4 ld_cluster_v4(uint32_t addr) {
   return v;
 }
 
+template <int OUT>
 __device__ __forceinline__ float activate_any(float v, int activation) {
   switch (activation) {
     case INT8CONV_ACT_RELU:
-      return activate<INT8CONV_ACT_RELU>(v);
+      return activate<INT8CONV_ACT_RELU, OUT == INT8CONV_FP32>(v);
     case INT8CONV_ACT_GELU:
-      return activate<INT8CONV_ACT_GELU>(v);
+      return activate<INT8CONV_ACT_GELU, OUT == INT8CONV_FP32>(v);
     case INT8CONV_ACT_GELU_TANH:
-      return activate<INT8CONV_ACT_GELU_TANH>(v);
+      return activate<INT8CONV_ACT_GELU_TANH, OUT == INT8CONV_FP32>(v);
     case INT8CONV_ACT_SILU:
-      return activate<INT8CONV_ACT_SILU>(v);
+      return activate<INT8CONV_ACT_SILU, OUT == INT8CONV_FP32>(v);
     default:
       return v;
   }
@@ -960,7 +961,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int32_t acc[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        float v = activate_any(fmaf(static_cast<float>(acc[j]) * cs[j], rs, b[j]), g.activation);
+        float v = activate_any<OUT>(fmaf(static_cast<float>(acc[j]) * cs[j], rs, b[j]), g.activation);
         v = OUT == INT8CONV_INT8 ? v * g.inv_out_scale : v + res[j];
         if (col + j < g.N) static_cast<T *>(g.y)[row * g.ldy + col + j] = Elem<OUT>::store(v);
       }
