@@ -48,6 +48,12 @@ __device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
+__device__ __forceinline__ uint64_t f2_neg(uint64_t a) {
+  float lo, hi;
+  f2_unpack(a, lo, hi);
+  return f2_pack(-lo, -hi);
+}
+
 // The hardware's 2^x and 1/x, two units in the last place, denormals as zeros.
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;

@@ -20,10 +20,10 @@
 // chunks are joined as (mean, squared deviations) in a fixed order, so the result
 // does not depend on timing.
 //
-// Measured: 256 images of 3136 x 256 int32 to fp16 314 us, DRAM at 6.4 TB/s with x
+// Measured: 256 images of 3136 x 256 int32 to fp16 317 us, DRAM at 6.4 TB/s with x
 // read twice; 8 of 4096 x 320 bf16 to bf16 with silu 19 us, two kernels bound by
 // the latency of their loads and reductions (and, with silu, by the two special
-// functions of each element); one of 196 x 256 int32 6.8 us, where a launch alone
+// functions of each element); one of 196 x 256 int32 6.9 us, where a launch alone
 // takes 2.3.
 #include <cuda_runtime.h>
 #include <math.h>
@@ -210,27 +210,33 @@ __device__ __forceinline__ int rows_of(const NormArgs &a, int span) {
 
 // Batches of a run: a thread adds the squares of this many batches before it adds
 // the run's sum to the runs' before it.
-constexpr int kRun = 16;
+constexpr int kRun = 16;   // 32, 64 or 128 pixels
 
 // (mean, squared deviations) of every channel over pixels [0, rows) of x, this
 // CTA's span, into ch.m and ch.w.  `mine`: the parameters of channel threadIdx.x.
 //
 // A thread sums d = x - shift and d^2 of its own pixels, the shift its first
-// pixel.  After 1, 2, 4 and so on up to kRun batches, and after every run from
-// then on, the shift moves to the mean so far, the sums with it:
+// pixel.  Where it has more than 16 (and a batch), the shift moves to the mean so
+// far after 8 pixels, 32, twice that up to a run, and every further run, the sums
+// with it:
 //   e = s1 / n,  s2 <- s2 - e (2 s1 - n e),  s1 <- s1 - n e,  shift <- shift + e
-// No step cancels, wherever an outlier lies: the shift is one of the values or
-// the mean of at least half of them, so the squares about it are at most n times
-// the squared deviations in the first batch (n <= 8), and later at most twice.
-// The longest chain of additions of squares is kRun batches, then the runs.  A
-// thread's squares of finished runs lie in its `cell`, which is free until the
-// sums are joined.  SCALED: each value times its channel's scale.
+// No step cancels, wherever an outlier lies: the shift is the mean of a part of
+// the values, and the squares about the mean of m of n values are at most n / m
+// times the squared deviations: up to 24 where that is all (16 and a batch), 8 in
+// the first 8, 4 from there to 32, and from then on 2.  The longest chain of
+// additions of squares is a run (32 to 128), then the runs.  A thread's squares of
+// finished runs lie in its `cell`, which is free until the sums are joined.
+// SCALED: each value times its channel's scale.
+//
+// On small images what is executed once counts by its length (the instructions
+// come from L2): the sums move as pairs.
 template <int DT, int VEC, bool SCALED>
 __device__ __forceinline__ void span_sums(const NormArgs &a, const typename Elem<DT>::type *x,
                                           int rows, uint8_t *area, float *cell,
                                           const Channels &ch, const Params &mine) {
   using T = typename Elem<DT>::type;
   constexpr int kBatch = batch<DT, VEC>();
+  constexpr int kPairs = (VEC + 1) / 2;   // one channel alone: the pair's other half is 0
   const int cols = a.channels / VEC;
   uint4 *slot = reinterpret_cast<uint4 *>(area);
   int kept = a.keep;   // full batches go to shared memory until this many vectors lie there
@@ -239,10 +245,30 @@ __device__ __forceinline__ void span_sums(const NormArgs &a, const typename Elem
     const bool active = k.part < k.lanes;
     const int wide = k.width * VEC, c0 = col0 * VEC;
     float *own = cell + k.part * wide + k.col * VEC;   // this thread's place (active threads)
-    const int pixels = active && k.part < rows ? (rows - k.part - 1) / k.lanes + 1 : 0;
-    float x0[VEC], s1[VEC], s2[VEC];
+    // The first `more` threads of a column hold one pixel more than the others.
+    const int each = rows / k.lanes, more = rows - each * k.lanes;
+    const int pixels = active ? each + (k.part < more ? 1 : 0) : 0;
+    uint64_t x0[kPairs], s1[kPairs], s2[kPairs];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) x0[j] = s1[j] = s2[j] = 0.f;
+    for (int j = 0; j < kPairs; ++j) x0[j] = s1[j] = s2[j] = 0;
+    auto put = [&](const uint64_t (&v)[kPairs]) {
+      float f[2 * kPairs];
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) f2_unpack(v[j], f[2 * j], f[2 * j + 1]);
+      if constexpr (VEC == 1)
+        own[0] = f[0];
+      else
+        put_vec<VEC>(own, f);
+    };
+    auto add_own = [&](uint64_t (&v)[kPairs]) {
+      float f[2 * kPairs] = {};
+      if constexpr (VEC == 1)
+        f[0] = own[0];
+      else
+        get_vec<VEC>(own, f);
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) v[j] = f2_add(v[j], f2_pack(f[2 * j], f[2 * j + 1]));
+    };
     if (pixels > 0) {
       [[maybe_unused]] float by[VEC];
       if constexpr (SCALED) {
@@ -251,54 +277,58 @@ __device__ __forceinline__ void span_sums(const NormArgs &a, const typename Elem
       }
       const T *at = x + (col0 + k.col) * VEC + k.part * a.ldx;
       const int64_t step = k.lanes * a.ldx;
-      auto add = [&](const Raw<DT, VEC> &r) {
-        if constexpr (VEC == 1) {
-          const float d = SCALED ? fmaf(r.get(0), by[0], -x0[0]) : r.get(0) - x0[0];
-          s1[0] += d;
-          s2[0] = fmaf(d, d, s2[0]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < VEC; j += 2) {
-            const uint64_t minus = f2_pack(-x0[j], -x0[j + 1]);
-            uint64_t d;
-            if constexpr (SCALED)
-              d = f2_fma(r.pair(j), f2_pack(by[j], by[j + 1]), minus);
-            else
-              d = f2_add(r.pair(j), minus);
-            f2_unpack(f2_add(f2_pack(s1[j], s1[j + 1]), d), s1[j], s1[j + 1]);
-            f2_unpack(f2_fma(d, d, f2_pack(s2[j], s2[j + 1])), s2[j], s2[j + 1]);
-          }
-        }
+      auto pair = [&](const Raw<DT, VEC> &r, int j) {
+        if constexpr (VEC == 1)
+          return f2_pack(r.get(0), 0.f);
+        else
+          return r.pair(2 * j);
+      };
+      auto times = [&](int j) {
+        if constexpr (!SCALED)
+          return f2_pack(1.f, 1.f);
+        else if constexpr (VEC == 1)
+          return f2_pack(by[0], 0.f);
+        else
+          return f2_pack(by[2 * j], by[2 * j + 1]);
       };
       auto start = [&](const Raw<DT, VEC> &r) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          x0[j] = r.get(j);
-          if constexpr (SCALED) x0[j] *= by[j];
+        for (int j = 0; j < kPairs; ++j)
+          x0[j] = SCALED ? f2_mul(pair(r, j), times(j)) : pair(r, j);
+      };
+      auto add = [&](const Raw<DT, VEC> &r) {
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          const uint64_t minus = f2_neg(x0[j]);
+          const uint64_t d = SCALED ? f2_fma(pair(r, j), times(j), minus) : f2_add(pair(r, j), minus);
+          s1[j] = f2_add(s1[j], d);
+          s2[j] = f2_fma(d, d, s2[j]);
         }
       };
       // The sums of n pixels move to their mean (to any value near it: the sums
       // are exact about the shift, whatever it is).
       auto center = [&](float n) {
-        const float inv = rcp_approx(n);
+        const float i = rcp_approx(n);
+        const uint64_t inv = f2_pack(i, i), minus_n = f2_pack(-n, -n);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float to = fmaf(s1[j], inv, x0[j]);
-          const float e = to - x0[j];
-          const float rest = fmaf(-n, e, s1[j]);
-          s2[j] = fmaf(-e, s1[j] + rest, s2[j]);
+        for (int j = 0; j < kPairs; ++j) {
+          const uint64_t to = f2_fma(s1[j], inv, x0[j]);
+          const uint64_t e = f2_add(to, f2_neg(x0[j]));
+          const uint64_t rest = f2_fma(minus_n, e, s1[j]);
+          s2[j] = f2_fma(f2_neg(e), f2_add(s1[j], rest), s2[j]);
           s1[j] = rest;
           x0[j] = to;
         }
       };
-      int left = pixels, done = 0, until = 1;   // batches done, and when to center next
-      int centered = 1;                         // pixels of the sums when last centered
+      constexpr int kRunPixels = kRun * kBatch;
+      int left = pixels;
+      int mark = pixels > 16 + kBatch ? pixels - 8 : -1;   // center where `left` is this
 #pragma unroll 1
-      for (; left >= kBatch; left -= kBatch) {
+      while (left >= kBatch) {
         Raw<DT, VEC> r[kBatch];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u, at += step) r[u].load(at);
-        if (done == 0) start(r[0]);
+        if (left == pixels) start(r[0]);
         if constexpr (VEC > 1) {
           if (kept > 0) {
 #pragma unroll
@@ -309,19 +339,19 @@ __device__ __forceinline__ void span_sums(const NormArgs &a, const typename Elem
         }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) add(r[u]);
-        if (++done == until) {
-          if (done > kRun) {
+        left -= kBatch;
+        if (left == mark) {
+          const int n = pixels - left;
+          if (n > kRunPixels) add_own(s2);
+          center(static_cast<float>(n));
+          if (n < kRunPixels) {
+            mark = pixels - (n == 8 ? 32 : 2 * n);
+          } else {
+            put(s2);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s2[j] += own[j];
+            for (int j = 0; j < kPairs; ++j) s2[j] = 0;
+            mark -= kRunPixels;
           }
-          center(static_cast<float>(done * kBatch));
-          centered = done * kBatch;
-          if (done >= kRun) {
-            put_vec<VEC>(own, s2);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) s2[j] = 0.f;
-          }
-          until += done < kRun ? done : kRun;
         }
       }
 #pragma unroll 1
@@ -331,32 +361,28 @@ __device__ __forceinline__ void span_sums(const NormArgs &a, const typename Elem
         if (left == pixels) start(r);
         add(r);
       }
-      if (done >= kRun) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s2[j] += own[j];
-      }
+      if (pixels >= kRunPixels) add_own(s2);
       // Now the mean, and the squares about it: less those of what its rounding
       // left, the squared deviations.
-      if (pixels > centered) center(static_cast<float>(pixels));
-      const float inv = rcp_approx(static_cast<float>(pixels));
+      if (pixels > 1) {
+        const float n = static_cast<float>(pixels);
+        center(n);
+        const float i = -rcp_approx(n);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) s2[j] = fmaf(-s1[j] * inv, s1[j], s2[j]);
+        for (int j = 0; j < kPairs; ++j)
+          s2[j] = f2_fma(f2_mul(s1[j], f2_pack(i, i)), s1[j], s2[j]);
+      }
     }
     // The threads of a column join: first the means, relative to the first
-    // thread's, then the squared deviations about the mean of all.  The first
-    // `more` threads hold one pixel more than the others.
-    const int each = rows / k.lanes, more = rows - each * k.lanes;
-    auto gather = [&](const float (&v)[VEC]) {
-      if (active) put_vec<VEC>(own, v);
-      __syncthreads();
-    };
-    gather(x0);
+    // thread's, then the squared deviations about the mean of all.
+    if (active) put(x0);
+    __syncthreads();
     const float inv = 1.f / static_cast<float>(rows > 0 ? rows : 1);
 #pragma unroll 1
     for (int i = threadIdx.x; i < wide; i += kThreads) {
       const float ref = cell[i];
       float all = 0.f, head = 0.f;
-#pragma unroll 8
+#pragma unroll 4
       for (int q = 0; q < k.lanes; ++q) {
         const float d = cell[q * wide + i] - ref;
         all += d;
@@ -368,22 +394,26 @@ __device__ __forceinline__ void span_sums(const NormArgs &a, const typename Elem
     __syncthreads();
     if (pixels > 0) {
       const float n = static_cast<float>(pixels);
-      float mean[VEC];
-      get_vec<VEC>(ch.m + c0 + k.col * VEC, mean);
+      float mean[2 * kPairs] = {};
+      if constexpr (VEC == 1)
+        mean[0] = ch.m[c0 + k.col];
+      else
+        get_vec<VEC>(ch.m + c0 + k.col * VEC, mean);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float d = x0[j] - mean[j];
-        // s2 is not below zero but for a rounding; NaN stays NaN.
-        s2[j] = fmaf(d * n, d, s2[j] < 0.f ? 0.f : s2[j]);
+      for (int j = 0; j < kPairs; ++j) {
+        const uint64_t d = f2_add(x0[j], f2_pack(-mean[2 * j], -mean[2 * j + 1]));
+        s2[j] = f2_fma(f2_mul(d, f2_pack(n, n)), d, s2[j]);
       }
     }
-    gather(s2);
+    if (active) put(s2);
+    __syncthreads();
 #pragma unroll 1
     for (int i = threadIdx.x; i < wide; i += kThreads) {
       const int c = c0 + i;
       float sq = 0.f;
-#pragma unroll 8
+#pragma unroll 4
       for (int q = 0; q < k.lanes; ++q) sq += cell[q * wide + i];
+      if (sq < 0.f) sq = 0.f;   // a rounding's; NaN stays NaN
       if constexpr (SCALED) {
         ch.w[c] = sq;
       } else {
@@ -397,14 +427,11 @@ __device__ __forceinline__ void span_sums(const NormArgs &a, const typename Elem
 }
 
 // The same of every group, into part[].
-template <int DT, int VEC>
+template <int DT, int VEC, bool SCALED>
 __device__ __forceinline__ void span_stats(const NormArgs &a, const typename Elem<DT>::type *x,
                                            int rows, uint8_t *area, float *cell,
                                            const Channels &ch, const Params &mine, float2 *part) {
-  if (DT != INT8CONV_INT32 && a.scale != nullptr)
-    span_sums<DT, VEC, DT != INT8CONV_INT32>(a, x, rows, area, cell, ch, mine);
-  else
-    span_sums<DT, VEC, false>(a, x, rows, area, cell, ch, mine);
+  span_sums<DT, VEC, SCALED>(a, x, rows, area, cell, ch, mine);
   // Channels of a group all hold `rows` values: the mean of means (relative to
   // the first, so that a large mean costs no bits), and the squares plus `rows`
   // times the means' squared deviations.  2 to 32 lanes share a group.
@@ -573,7 +600,7 @@ __device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
 constexpr int kMaxCluster = 8;
 
 // One kernel: the CTAs of a cluster share an image.
-template <int DT, int OUT, int VEC>
+template <int DT, int OUT, int VEC, bool SCALED>
 __global__ void __launch_bounds__(kThreads, 2) norm_cluster_kernel(const NormArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   using T = typename Elem<DT>::type;
@@ -590,8 +617,8 @@ __global__ void __launch_bounds__(kThreads, 2) norm_cluster_kernel(const NormArg
   const int rows = rows_of(a, span);
   const int64_t first = image * a.pixels + static_cast<int64_t>(span) * a.span_pixels;
   const T *x = static_cast<const T *>(a.x) + first * a.ldx;
-  span_stats<DT, VEC>(a, x, rows, smem, reinterpret_cast<float *>(smem + plan.cell_off), ch, mine,
-                      part);
+  span_stats<DT, VEC, SCALED>(a, x, rows, smem, reinterpret_cast<float *>(smem + plan.cell_off), ch,
+                              mine, part);
   cluster_sync_all();
   // 8 lanes share a group, one for each CTA of the cluster.
   const int k = threadIdx.x & (kMaxCluster - 1);
@@ -621,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_cluster_kernel(const NormArg
 }
 
 // Two kernels, the first: statistics of one chunk of pixels.
-template <int DT, int VEC>
+template <int DT, int VEC, bool SCALED>
 __global__ void __launch_bounds__(kThreads, 2) norm_stats_kernel(const NormArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   using T = typename Elem<DT>::type;
@@ -634,8 +661,9 @@ __global__ void __launch_bounds__(kThreads, 2) norm_stats_kernel(const NormArgs 
   const int64_t image = blockIdx.x / a.spans;
   const int span = static_cast<int>(blockIdx.x) % a.spans;
   const int64_t first = image * a.pixels + static_cast<int64_t>(span) * a.span_pixels;
-  span_stats<DT, VEC>(a, static_cast<const T *>(a.x) + first * a.ldx, rows_of(a, span), smem,
-                      reinterpret_cast<float *>(smem + plan.cell_off), ch, mine, part);
+  span_stats<DT, VEC, SCALED>(a, static_cast<const T *>(a.x) + first * a.ldx, rows_of(a, span),
+                              smem, reinterpret_cast<float *>(smem + plan.cell_off), ch, mine,
+                              part);
   __syncthreads();
   for (int g = threadIdx.x; g < a.groups; g += kThreads)
     a.partial[(image * a.groups + g) * a.spans + span] = part[g];
@@ -686,30 +714,33 @@ struct NormKernels {
   const void *cluster, *stats, *apply;
 };
 
-template <int DT, int OUT, int VEC>
+template <int DT, int OUT, int VEC, bool SCALED>
 NormKernels kernels_of() {
-  return NormKernels{reinterpret_cast<const void *>(&norm_cluster_kernel<DT, OUT, VEC>),
-                     reinterpret_cast<const void *>(&norm_stats_kernel<DT, VEC>),
+  return NormKernels{reinterpret_cast<const void *>(&norm_cluster_kernel<DT, OUT, VEC, SCALED>),
+                     reinterpret_cast<const void *>(&norm_stats_kernel<DT, VEC, SCALED>),
                      reinterpret_cast<const void *>(&norm_apply_kernel<DT, OUT, VEC>)};
 }
 
-template <int DT, int VEC>
+template <int DT, int VEC, bool SCALED>
 NormKernels kernels_for_out(int out) {
   switch (out) {
     case INT8CONV_BF16:
-      return kernels_of<DT, INT8CONV_BF16, VEC>();
+      return kernels_of<DT, INT8CONV_BF16, VEC, SCALED>();
     case INT8CONV_FP16:
-      return kernels_of<DT, INT8CONV_FP16, VEC>();
+      return kernels_of<DT, INT8CONV_FP16, VEC, SCALED>();
     case INT8CONV_FP32:
-      return kernels_of<DT, INT8CONV_FP32, VEC>();
+      return kernels_of<DT, INT8CONV_FP32, VEC, SCALED>();
     default:
-      return kernels_of<DT, INT8CONV_INT8, VEC>();
+      return kernels_of<DT, INT8CONV_INT8, VEC, SCALED>();
   }
 }
 
 template <int DT>
-NormKernels kernels_for(bool vec, int out) {
-  return vec ? kernels_for_out<DT, 8>(out) : kernels_for_out<DT, 1>(out);
+NormKernels kernels_for(bool vec, bool scaled, int out) {
+  if constexpr (DT != INT8CONV_INT32) {   // int32 takes its scale after the sums
+    if (scaled) return vec ? kernels_for_out<DT, 8, true>(out) : kernels_for_out<DT, 1, true>(out);
+  }
+  return vec ? kernels_for_out<DT, 8, false>(out) : kernels_for_out<DT, 1, false>(out);
 }
 
 // How a call runs: spans of an image, and whether they are one cluster.
@@ -789,10 +820,12 @@ int8conv_status launch_group_norm_impl(const int8conv_group_norm &d, const void 
   const bool vec = d.channels % 8 == 0 && (d.ldx * xs) % 16 == 0 && (d.ldy * ys) % ya == 0 &&
                    (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
                    (reinterpret_cast<uintptr_t>(y) & (ya - 1)) == 0;
-  const NormKernels kernels = d.x_dtype == INT8CONV_BF16   ? kernels_for<INT8CONV_BF16>(vec, d.y_dtype)
-                              : d.x_dtype == INT8CONV_FP16 ? kernels_for<INT8CONV_FP16>(vec, d.y_dtype)
-                              : d.x_dtype == INT8CONV_FP32 ? kernels_for<INT8CONV_FP32>(vec, d.y_dtype)
-                                                           : kernels_for<INT8CONV_INT32>(vec, d.y_dtype);
+  const bool scaled = d.scale != nullptr;
+  const NormKernels kernels =
+      d.x_dtype == INT8CONV_BF16   ? kernels_for<INT8CONV_BF16>(vec, scaled, d.y_dtype)
+      : d.x_dtype == INT8CONV_FP16 ? kernels_for<INT8CONV_FP16>(vec, scaled, d.y_dtype)
+      : d.x_dtype == INT8CONV_FP32 ? kernels_for<INT8CONV_FP32>(vec, scaled, d.y_dtype)
+                                   : kernels_for<INT8CONV_INT32>(vec, scaled, d.y_dtype);
   const int width = vec ? 8 : 1;
   LaunchPlan plan;
   plan.block = dim3(kThreads);

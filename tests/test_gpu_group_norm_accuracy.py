@@ -25,10 +25,13 @@ def _exact(x, groups, scale=None):
 def _tolerance(z, mean, size, p, c, vec):
     """Half an fp32 step is u.  A run of a thread is at most 128 positions.
 
-    Variance: the squares added are never more than twice what they come to (8
-    times in a first batch of 8), so its relative error is the additions' chain:
-    2 * (128 + runs) + 64 of a thread, up to `lanes` threads of a column, 32
-    steps over channels and CTAs.  Half of it reaches 1 / deviation.
+    Variance: adding the k-th of n squares about a shift that is the mean of m of
+    them costs u times a sum of at most n / m times what they come to, on average
+    half of it.  A thread with up to 24 positions: 24 * 24 / 2.  With more: 8 * 8 / 2
+    up to 8, 24 * 4 / 2 up to 32, 96 * 2 / 2 up to the first run, 128 in the runs
+    and 2 for each; all below 2 * (128 + runs) + 64.  Then up to `lanes`
+    threads of a column, 32 steps over channels and CTAs.  Half of the relative
+    error reaches 1 / deviation.
     Mean, in deviations: a run's sum starts near zero, so 128 steps of the
     values' mean distance (below 1.5 deviations, 200 in all); the threads' means
     relative to the first one's, which may be sqrt(lanes) deviations away, over
