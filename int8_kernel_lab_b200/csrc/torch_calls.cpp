@@ -4,9 +4,10 @@
 // operators.py checks its arguments through some forty attribute reads, which
 // take longer than the smallest kernels.  These functions make the same checks
 // on the tensors themselves, allocate the result and launch; they return None,
-// having done nothing, for every call that is not plainly in order, and
-// operators.py then finds out what is wrong with it, or handles it.  There is no
-// computation here.  The pointers, sizes and pitches that reach the library are
+// having launched nothing, for every call that is not plainly in order, and
+// operators.py then finds out what is wrong with it, or handles it.  A launch
+// that failed is reported at once (on_failure): it is not tried again, since a
+// call may add to its own output.  There is no computation here.  The pointers, sizes and pitches that reach the library are
 // the same either way.
 #include <Python.h>
 
@@ -103,6 +104,26 @@ void *stream_of(int device) { return c10::cuda::getCurrentCUDAStream(device).str
 
 PyObject *declined() { Py_RETURN_NONE; }
 
+// operators.py's report of a status: raises.
+PyObject *report = nullptr;
+
+PyObject *on_failure(PyObject *, PyObject *callable) {
+  Py_INCREF(callable);
+  Py_XSETREF(report, callable);
+  Py_RETURN_NONE;
+}
+
+// What a call returns whose launch had another status than OK: None for those
+// that the library's checks of arguments give, before anything is launched.
+PyObject *refused(int8conv_status st, const char *what) {
+  if (st == INT8CONV_BAD_ARGUMENT || st == INT8CONV_BAD_POINTER || report == nullptr)
+    return declined();
+  PyObject *r = PyObject_CallFunction(report, "is", static_cast<int>(st), what);
+  Py_XDECREF(r);
+  if (r != nullptr) PyErr_Format(PyExc_RuntimeError, "%s: status %d", what, static_cast<int>(st));
+  return nullptr;
+}
+
 // (a, b, offsets, y, row_scale, col_scale, bias, residual, activation, dtype, out_scale)
 // -> y, or None.  offsets None: the plain product.  y None: a new result of type `dtype`.
 PyObject *matmul(PyObject *, PyObject *const *args, Py_ssize_t count) {
@@ -190,7 +211,7 @@ PyObject *matmul(PyObject *, PyObject *const *args, Py_ssize_t count) {
                                                 static_cast<int32_t>(groups), my.p, stream)
                : int8conv_launch_matmul(&d, pa, pb, my.p, stream);
   Py_END_ALLOW_THREADS
-  if (st != INT8CONV_OK) return declined();
+  if (st != INT8CONV_OK) return refused(st, grouped ? "grouped_matmul" : "matmul");
   return THPVariable_Wrap(std::move(y));
   END_HANDLE_TH_ERRORS
 }
@@ -229,7 +250,7 @@ PyObject *quantize_rows(PyObject *, PyObject *const *args, Py_ssize_t count) {
                                      static_cast<const int32_t *>(pi), static_cast<int8_t *>(mq.p),
                                      mq.pitch, static_cast<float *>(scale.data_ptr()), stream);
   Py_END_ALLOW_THREADS
-  if (st != INT8CONV_OK) return declined();
+  if (st != INT8CONV_OK) return refused(st, "quantize_rows");
   PyObject *pair = PyTuple_New(2);
   if (pair == nullptr) return nullptr;
   PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(q)));
@@ -318,7 +339,7 @@ PyObject *group_norm(PyObject *, PyObject *const *args, Py_ssize_t count) {
   Py_BEGIN_ALLOW_THREADS
   st = int8conv_launch_group_norm(&d, px.p, py.p, ws, bytes, stream);
   Py_END_ALLOW_THREADS
-  if (st != INT8CONV_OK) return declined();
+  if (st != INT8CONV_OK) return refused(st, "group_norm");
   return THPVariable_Wrap(std::move(y));
   END_HANDLE_TH_ERRORS
 }
@@ -332,6 +353,7 @@ PyMethodDef methods[] = {
     {"matmul", fast(&matmul), METH_FASTCALL, nullptr},
     {"quantize_rows", fast(&quantize_rows), METH_FASTCALL, nullptr},
     {"group_norm", fast(&group_norm), METH_FASTCALL, nullptr},
+    {"on_failure", &on_failure, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -51,6 +51,7 @@ def _load_calls():
     spec = importlib.util.spec_from_file_location("torch_calls", _CALLS_PATH)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
+    module.on_failure(_abi.check)
     return module
 
 
