@@ -296,7 +296,8 @@ PyObject *group_norm(PyObject *, PyObject *const *args, Py_ssize_t count) {
   const int device = c10::cuda::current_device();
   Pixels px, py;
   int8conv_group_norm d{};
-  if (!pixels(x, device, px)) return declined();
+  // The descriptor's channels are 32 bits wide.
+  if (!pixels(x, device, px) || px.c > INT8CONV_MAX_NORM_CHANNELS) return declined();
   const void *gamma = nullptr, *beta = nullptr, *scale = nullptr;
   if (!vector(args[2], at::kFloat, px.c, device, &gamma) ||
       !vector(args[3], at::kFloat, px.c, device, &beta) ||

@@ -95,6 +95,13 @@ def _dtype_code(dtype) -> int:
     return code
 
 
+def _pack(descriptor: struct.Struct, *fields) -> bytes:
+    try:
+        return descriptor.pack(*fields)
+    except struct.error as e:
+        raise ValueError(f"an argument is out of range: {e}") from None
+
+
 def _activation(name: str) -> int:
     code = _abi.ACTIVATIONS.get(name)
     if code is None:
@@ -179,11 +186,11 @@ def _describe(m, k, lda, n, bk, ldb, y, row_scale, col_scale, bias, activation, 
         res_ptr, rm, rn, ldr = _matrix("residual", residual, device)
         if rm != m or rn != n:
             _fail("residual", f"a {m} x {n} matrix", residual)
-    return _MATMUL.pack(m, n, k, lda, ldb, ldy, ldr,
-                        _vector("row_scale", row_scale, m, device),
-                        _vector("col_scale", col_scale, n * groups, device),
-                        _vector("bias", bias, n * groups, device), res_ptr,
-                        _activation(activation), code, _out_step(code, out_scale)), y_ptr
+    return _pack(_MATMUL, m, n, k, lda, ldb, ldy, ldr,
+                 _vector("row_scale", row_scale, m, device),
+                 _vector("col_scale", col_scale, n * groups, device),
+                 _vector("bias", bias, n * groups, device), res_ptr,
+                 _activation(activation), code, _out_step(code, out_scale)), y_ptr
 
 
 def launch_matmul(a, b, y, *, row_scale=None, col_scale=None, bias=None, activation: str = "none",
@@ -387,10 +394,10 @@ def _norm_desc(x, groups, y, gamma, beta, eps, activation, scale, out_scale, dev
         _fail("y", f"a tensor of shape {tuple(x.shape)}", y)
     y_ptr, _, _, _, ldy = _pixels("y", y, device)
     code = _dtype_code(y.dtype)
-    return _NORM.pack(n, pixels, c, int(groups), ldx, ldy, _vector("scale", scale, c, device),
-                      _vector("gamma", gamma, c, device), _vector("beta", beta, c, device),
-                      float(eps), _activation(activation), _dtype_code(x.dtype), code,
-                      _out_step(code, out_scale)), x_ptr, y_ptr
+    return _pack(_NORM, n, pixels, c, int(groups), ldx, ldy, _vector("scale", scale, c, device),
+                 _vector("gamma", gamma, c, device), _vector("beta", beta, c, device),
+                 float(eps), _activation(activation), _dtype_code(x.dtype), code,
+                 _out_step(code, out_scale)), x_ptr, y_ptr
 
 
 def group_norm_workspace_bytes(x, groups: int, y) -> int:
