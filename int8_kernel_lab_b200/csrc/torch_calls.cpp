@@ -363,4 +363,19 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "torch_calls", nullptr, -1, methods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_torch_calls(void) { return PyModule_Create(&module); }
+#ifndef BUILT_FOR_TORCH
+#define BUILT_FOR_TORCH "unknown"
+#endif
+#define TEXT_OF(x) #x
+#define VERSION_TEXT(major, minor) TEXT_OF(major) "." TEXT_OF(minor)
+
+// Nothing of torch is touched here: operators.py compares `built_for` with what
+// runs before it calls anything.
+PyMODINIT_FUNC PyInit_torch_calls(void) {
+  PyObject *m = PyModule_Create(&module);
+  if (m != nullptr &&
+      PyModule_AddStringConstant(m, "built_for", "torch " BUILT_FOR_TORCH ", Python " VERSION_TEXT(
+                                     PY_MAJOR_VERSION, PY_MINOR_VERSION)) != 0)
+    Py_CLEAR(m);
+  return m;
+}

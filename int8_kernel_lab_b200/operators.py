@@ -27,7 +27,7 @@ from . import _abi
 
 # One short call to the GPU takes a few microseconds.  The calls that allocate
 # their result and run on the current stream therefore go through torch_calls
-# (csrc/torch_calls.cpp, where it was built), which checks and launches a
+# (csrc/torch_calls.cpp, where it was built for this torch and Python), which checks and launches a
 # well-formed call in about one microsecond beside the launch itself and
 # declines every other; what it declines, and every other call, takes the
 # checks below, which name what is wrong.  They too are written to cost little:
@@ -42,15 +42,28 @@ _raw_stream = None
 _calls = None
 
 
-def _load_calls():
-    """The compiled calls, or None where they were not built."""
+def _load_calls(torch):
+    """The compiled calls; None where they were not built, and, with a warning,
+    where they were built for another torch or Python: they read its tensors as
+    they lie in memory.  The checks in Python need no such match."""
     if not _CALLS_PATH.exists():
         return None
     import importlib.util
+    import sys
+    import warnings
 
-    spec = importlib.util.spec_from_file_location("torch_calls", _CALLS_PATH)
-    module = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(module)
+    here = f"torch {torch.__version__}, Python {sys.version_info[0]}.{sys.version_info[1]}"
+    try:
+        spec = importlib.util.spec_from_file_location("torch_calls", _CALLS_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        wrong = "" if module.built_for == here else f"was built for {module.built_for}"
+    except (ImportError, OSError, AttributeError) as e:
+        wrong = f"does not load ({e})"
+    if wrong:
+        warnings.warn(f"{_CALLS_PATH} {wrong}, this is {here}: the operators' calls take longer "
+                      "until it is built again", RuntimeWarning, stacklevel=2)
+        return None
     module.on_failure(_abi.check)
     return module
 
@@ -59,8 +72,7 @@ def _load_torch():
     global _torch, _raw_stream, _calls
     import torch
 
-    _calls = _load_calls()
-
+    _calls = _load_calls(torch)
     _DTYPES.update({getattr(torch, name): code for name, code in _abi.DTYPES.items()})
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     _torch = torch
