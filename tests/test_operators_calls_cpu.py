@@ -1,7 +1,10 @@
 """Loading the compiled calls: only those built for the torch and Python that run,
 and without them the operators go on through the checks in Python."""
+import importlib.util
+import subprocess
 import sys
 import warnings
+from pathlib import Path
 
 import pytest
 import torch
@@ -53,3 +56,23 @@ def test_missing_file_is_not_worth_a_warning(fresh, tmp_path):
         warnings.simplefilter("error")
         operators._load_torch()
     assert operators._calls is None
+
+
+def _commands(*variables):
+    """What make would run for everything, from the start."""
+    csrc = Path(m.__file__).parent / "csrc"
+    return subprocess.run(["make", "-n", "-B", "-C", str(csrc), f"PYTHON={sys.executable}", *variables],
+                          capture_output=True, text=True, check=True).stdout
+
+
+def test_library_builds_without_a_torch_that_has_cuda(tmp_path):
+    torch_dir = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    assert ("torch_calls.so" in _commands()) == (torch_dir / "lib" / "libc10_cuda.so").exists()
+    # A CPU build of torch: libc10, its headers, no libc10_cuda.
+    (tmp_path / "lib").mkdir()
+    (tmp_path / "lib" / "libc10.so").touch()
+    (tmp_path / "include" / "c10" / "cuda").mkdir(parents=True)
+    (tmp_path / "include" / "c10" / "cuda" / "CUDAStream.h").touch()
+    for where in (tmp_path, tmp_path / "none", ""):
+        out = _commands(f"TORCH={where}")
+        assert "libint8conv.so" in out and "torch_calls.cpp" not in out
