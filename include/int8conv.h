@@ -254,6 +254,12 @@ int8conv_status int8conv_launch_grouped_matmul(const int8conv_matmul *desc, cons
                                                const int32_t *offsets, int32_t groups, void *y,
                                                void *stream);
 
+/* How a product of these sizes runs on a device with `sms` SMs (groups 0: the
+ * plain one), for tests: bits 0-15 the tile's columns, bit 16 CTA pairs, bit 17
+ * a column tile of b that stays in shared memory, bits 20-23 the CTAs that share
+ * k.  0 for sizes outside the ranges above.  Results do not depend on it. */
+int32_t int8conv_debug_matmul_form(int64_t m, int64_t n, int64_t k, int32_t groups, int32_t sms);
+
 /* Rows of x to int8 with one scale each:
  *   scale[i] = max_k |x[r,k]| / 127
  *   q[i,k]   = round_half_even(x[r,k] / scale[i])       fp32, IEEE division

@@ -114,6 +114,8 @@ SIGNATURES = {
     "int8conv_launch_matmul": (ctypes.c_int, [_P] * 5),
     "int8conv_launch_grouped_matmul": (ctypes.c_int, [_P, _P, _P,
                                                       ctypes.c_int64, _P, ctypes.c_int32, _P, _P]),
+    "int8conv_debug_matmul_form": (ctypes.c_int32, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                                                    ctypes.c_int32, ctypes.c_int32]),
     "int8conv_launch_quantize_rows": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
                                                      _P, ctypes.c_int64, ctypes.c_int64, _P, _P,
                                                      ctypes.c_int64, _P, _P]),

@@ -99,6 +99,13 @@ int8conv_status int8conv_launch_grouped_matmul(const int8conv_matmul *desc, cons
                                  static_cast<cudaStream_t>(stream));
 }
 
+int32_t int8conv_debug_matmul_form(int64_t m, int64_t n, int64_t k, int32_t groups, int32_t sms) {
+  if (m < 1 || m > kMaxRows || n < 1 || n > kMaxRows || k < 1 || k > INT8CONV_MAX_PRODUCT_K ||
+      groups < 0 || groups > INT8CONV_MAX_GROUPS || sms < 1)
+    return 0;
+  return i8c::matmul_form(m, n, k, groups, sms);
+}
+
 int8conv_status int8conv_launch_quantize_rows(int64_t m, int64_t k, int32_t x_dtype, const void *x,
                                               int64_t rows, int64_t ldx, const int32_t *index,
                                               int8_t *q, int64_t ldq, float *scale, void *stream) {

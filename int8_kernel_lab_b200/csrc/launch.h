@@ -156,6 +156,8 @@ int8conv_status launch_splitk_impl(const int8conv_shape &s, const int8_t *x, con
 int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, const int8_t *b,
                                    int64_t group_stride, const int32_t *offsets, int32_t groups,
                                    void *y, cudaStream_t stream);
+// The form that a product takes (int8conv_debug_matmul_form).
+int32_t matmul_form(int64_t m, int64_t n, int64_t k, int32_t groups, int sms);
 int8conv_status launch_quantize_rows_impl(int64_t m, int64_t k, int x_dtype, const void *x,
                                           int64_t rows, int64_t ldx, const int32_t *index,
                                           int8_t *q, int64_t ldq, float *scale,

@@ -1145,7 +1145,44 @@ bool aligned(const void *p, int64_t bytes) {
   return (reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes)) == 0;
 }
 
+// The tiles of one launch on a device of `sms` SMs.
+struct MatmulTiles {
+  int a_rows, box_rows;
+  TileChoice choice;
+};
+
+MatmulTiles choose_tiles(int64_t m, int64_t n, int64_t k, int32_t groups, int sms) {
+  const bool grouped = groups > 0;
+  MatmulTiles t;
+  t.a_rows = 8;
+  while (t.a_rows < kBlockM && t.a_rows < m) t.a_rows *= 2;
+  // Row tiles: exact for a plain product; grouped, those of experts that share
+  // the rows about evenly (the host does not know the offsets): half a tile of
+  // each is empty.
+  const auto row_tiles = [&](int64_t rows) -> double {
+    if (!grouped) return static_cast<double>((m + rows - 1) / rows);
+    const int64_t active = groups < m ? groups : m;
+    const double each = static_cast<double>(m) / active;
+    return active * fmax(1.0, each / rows + 0.5);
+  };
+  // Experts with few rows each: boxes of about that many rows.
+  t.box_rows = t.a_rows;
+  if (grouped) {
+    const int64_t each = (m + groups - 1) / groups;
+    while (t.box_rows > 8 && t.box_rows > each) t.box_rows /= 2;
+  }
+  t.choice = choose_tile(row_tiles(kBlockM), row_tiles(2 * kBlockM), n,
+                         static_cast<int>((k + kBlockK - 1) / kBlockK), t.box_rows, sms,
+                         static_cast<int>(m < kBlockM ? m : kBlockM), grouped);
+  return t;
+}
+
 }  // namespace
+
+int32_t matmul_form(int64_t m, int64_t n, int64_t k, int32_t groups, int sms) {
+  const TileChoice c = choose_tiles(m, n, k, groups, sms).choice;
+  return c.bn | (c.pair ? 1 << 16 : 0) | (c.resident ? 1 << 17 : 0) | c.splits << 20;
+}
 
 int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, const int8_t *b,
                                    int64_t group_stride, const int32_t *offsets, int32_t groups,
@@ -1157,25 +1194,10 @@ int8conv_status launch_matmul_impl(const int8conv_matmul &d, const int8_t *a, co
   g.M = static_cast<int32_t>(d.m);
   g.N = static_cast<int32_t>(d.n);
   g.kblocks = static_cast<int32_t>((d.k + kBlockK - 1) / kBlockK);
-  g.a_rows = 8;
-  while (g.a_rows < kBlockM && g.a_rows < d.m) g.a_rows *= 2;
-  // Row tiles: exact for a plain product; grouped, those of experts that share
-  // the rows about evenly (the host does not know the offsets): half a tile of
-  // each is empty.
-  const auto row_tiles = [&](int64_t rows) -> double {
-    if (!grouped) return static_cast<double>((d.m + rows - 1) / rows);
-    const int64_t active = groups < d.m ? groups : d.m;
-    const double each = static_cast<double>(d.m) / active;
-    return active * fmax(1.0, each / rows + 0.5);
-  };
-  // Experts with few rows each: boxes of about that many rows.
-  g.box_rows = g.a_rows;
-  if (grouped) {
-    const int64_t each = (d.m + groups - 1) / groups;
-    while (g.box_rows > 8 && g.box_rows > each) g.box_rows /= 2;
-  }
-  const TileChoice c = choose_tile(row_tiles(kBlockM), row_tiles(2 * kBlockM), d.n, g.kblocks,
-                                   g.box_rows, sms, g.M < kBlockM ? g.M : kBlockM, grouped);
+  const MatmulTiles tiles_of = choose_tiles(d.m, d.n, d.k, groups, sms);
+  g.a_rows = tiles_of.a_rows;
+  g.box_rows = tiles_of.box_rows;
+  const TileChoice c = tiles_of.choice;
   g.bn = c.bn;
   const int tile_rows = c.pair ? 2 * kBlockM : kBlockM;
   g.n_tiles = static_cast<int32_t>((d.n + g.bn - 1) / g.bn);
