@@ -6,7 +6,8 @@
 //   one kernel   a thread-block cluster of 1 to 8 CTAs holds an image: each CTA
 //                takes a span of pixels, keeps as much of it as fits in shared
 //                memory, and the CTAs exchange their groups' partial statistics
-//                through distributed shared memory.  DRAM sees x once.
+//                through distributed shared memory.  What was kept is read once,
+//                the rest of x again.
 //   two kernels  for few large images, whose clusters would leave SMs idle:
 //                statistics of pixel chunks to scratch, then the norm, reading
 //                x again (from L2 while it fits there).
@@ -21,10 +22,15 @@
 // does not depend on timing.
 //
 // Measured: 256 images of 3136 x 256 int32 to fp16 317 us, DRAM at 6.4 TB/s with x
-// read twice; 8 of 4096 x 320 bf16 to bf16 with silu 19 us, two kernels bound by
-// the latency of their loads and reductions (and, with silu, by the two special
-// functions of each element); one of 196 x 256 int32 6.9 us, where a launch alone
-// takes 2.3.
+// read twice (one CTA holds an image of 3.2 MB, of which it keeps 0.1); 8 of
+// 4096 x 320 bf16 to bf16 with silu 18.8 us, two kernels bound by the latency of
+// their loads and reductions (and, with silu, by the two special functions of each
+// element); one of 196 x 256 int32 6.7 us, where a launch alone takes 2.3.
+//
+// Two CTAs of 512 threads an SM leave a thread 64 registers, and the vector kernels
+// spill some, before and after their loops (bf16 to bf16, bytes stored / loaded a
+// thread: one kernel 108 / 92; two kernels 4 / 4 and 140 / 156, of which 12 loads a
+// warp were executed over 2 x 65536 x 256).
 #include <cuda_runtime.h>
 #include <math.h>
 
@@ -763,10 +769,13 @@ NormShape norm_shape(const int8conv_group_norm &d) {
   if (spans > d.pixels) spans = 1;
   NormShape s{true, spans, (d.pixels + spans - 1) / spans};
   // Few images with much for each CTA of such a cluster: two kernels over chunks
-  // of all images, one to four for each SM by what there is to read (8 images of
-  // 4096 x 320 bf16: 19.2 us, in clusters of 8 28.4; 1 image 9.9 and 24.6; 16 of
-  // 8192 x 256 50 and 91; but 10 of 1400 x 112 10.4 and 8.4, 32 of 4096 x 512
-  // 100 and 83).
+  // of all images (8 images of 4096 x 320 bf16: 19.2 us, in clusters of 8 28.4; 1
+  // image 9.9 and 24.6; 16 of 8192 x 256 50 and 91; but 10 of 1400 x 112 10.4 and
+  // 8.4, 32 of 4096 x 512 100 and 83).  One, two or four chunks for each of the 148
+  // SMs, by what there is to read (bf16 with silu, 148 / 296 / 592 chunks, us: 10 MB
+  // 13.7 / 14.6 / 24.2; 14 MB 19.3 / 22.8 / 25.0; 20 MB 24.4 / 18.9 / 26.9; 40 MB
+  // 42.0 / 29.0 / 36.5; 56 MB 56.8 / 49.7 / 52.0; 147 MB 133 / 126 / 112; one image
+  // of 98 MB 78 / 67 / 79).
   const int64_t each = bytes / spans;
   if ((d.n * spans < 96 && each > 64 * 1024) || (d.n * spans <= 148 && each > 256 * 1024)) {
     const int64_t all = total > (64 << 20) ? 592 : total > (19 << 20) ? 296 : 148;

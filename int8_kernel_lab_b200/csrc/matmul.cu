@@ -993,12 +993,15 @@ struct TileChoice {
 // 256 x bn in the same), its loads (a_rows rows of A and its share of B, 128
 // bytes each) come at about 72 bytes a cycle, and the issuer needs 285; the
 // slowest counts.  The epilogue of the tile before runs meanwhile, 5 cycles a
-// column and 400 for its latencies.  A pair loses about 2500 cycles between two
-// tiles and 3000 at the start.  The rates were fitted to 28 plain and grouped
-// shapes timed at every width, single, in pairs and with resident B: the choice
-// is within 5 % of the fastest on each, within 1 % on most (2048 x 4096 x 4096:
-// pairs of 256 columns 27.7 us, best of 15 27.7, worst 69; 32768 x 320 x 320:
-// resident, 160 columns, 11.0 us, not resident 11.9, worst 21.6).  Few tiles may
+// column and 400 for its latencies (those of a plain epilogue: gelu_tanh to int8
+// takes some 8000 for 256 columns, so with a costly activation and k of 2048 and
+// less it is the epilogue that counts, which this does not see).  A pair loses
+// about 2500 cycles between two tiles and 3000 at the start.  The rates were
+// fitted to plain and grouped shapes timed at every width, single, in pairs and
+// with resident B, 25 without an activation, two with gelu and one with gelu_tanh:
+// the choice is within 5 % of the fastest on each, within 1 % on most (2048 x 4096
+// x 4096: pairs of 256 columns 27.7 us, best of 15 27.7, worst 69; 32768 x 320 x
+// 320: resident, 160 columns, 11.0 us, not resident 11.9, worst 21.6).  Few tiles may
 // also share k (the split kernel): 1 x 4096 x 4096 in 4 shares of 128 columns
 // 5.9 us, unsplit 7.0; 8 x 4096 x 16384 10.3 and 20.5; 128 x 4096 x 4096 9.4 and
 // 7.4 (unsplit taken).
