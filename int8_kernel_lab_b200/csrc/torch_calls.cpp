@@ -7,7 +7,8 @@
 // having launched nothing, for every call that is not plainly in order, and
 // operators.py then finds out what is wrong with it, or handles it.  A launch
 // that failed is reported at once (on_failure): it is not tried again, since a
-// call may add to its own output.  There is no computation here.  The pointers, sizes and pitches that reach the library are
+// call may add to its own output.  There is no computation here.  The pointers,
+// sizes and pitches that reach the library are
 // the same either way.
 #include <Python.h>
 

@@ -27,12 +27,12 @@ from . import _abi
 
 # One short call to the GPU takes a few microseconds.  The calls that allocate
 # their result and run on the current stream therefore go through torch_calls
-# (csrc/torch_calls.cpp, where it was built for this torch and Python), which checks and launches a
-# well-formed call in about one microsecond beside the launch itself and
-# declines every other; what it declines, and every other call, takes the
-# checks below, which name what is wrong.  They too are written to cost little:
-# attributes are read once, descriptors are packed in one step, and torch is
-# looked up once.
+# (csrc/torch_calls.cpp, where it was built for this torch and Python), which
+# checks and launches a well-formed call in about one microsecond beside the
+# launch itself and declines every other; what it declines, and every other
+# call, takes the checks below, which name what is wrong.  They too are written
+# to cost little: attributes are read once, descriptors are packed in one step,
+# and torch is looked up once.
 _MATMUL = struct.Struct("7q4P2if4x")        # int8conv_matmul
 _NORM = struct.Struct("2q2i2q3Pf3if4x")     # int8conv_group_norm
 _CALLS_PATH = _abi.LIB_PATH.parent / "torch_calls.so"

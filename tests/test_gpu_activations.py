@@ -96,3 +96,28 @@ def test_int8_results_of_the_activations(cuda):
         # The activation, the rounded 1 / step and the product with it.
         off = (y.double()[0] - want).abs() - 0.5
         assert bool((off <= U * (_bound(v.double(), activation, False) + 3) * want.abs() + 1e-30).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16, torch.int8], ids=str)
+@pytest.mark.parametrize("rows", [1, 200])
+@pytest.mark.parametrize("activation", sorted(FORMULAS))
+def test_ends_of_the_range(cuda, activation, rows, dtype):
+    inf, most = float("inf"), torch.finfo(torch.float32).max
+    v = torch.tensor([float("nan"), inf, -inf, most, -most, 2.5e38, -2.5e38, 0.0, -1e5, 1e-45] + [1.0] * 6,
+                     device="cuda")
+    a = torch.zeros(rows, 16, dtype=torch.int8, device="cuda")
+    b = torch.zeros(16, 16, dtype=torch.int8, device="cuda")
+    y = m.matmul(a, b, bias=v, activation=activation, dtype=dtype,
+                 out_scale=0.5 if dtype == torch.int8 else None)
+    for row in (y[0], y[-1]):
+        if dtype == torch.int8:
+            assert row[:9].tolist() == [0, 127, 0, 127, 0, 127, 0, 0, 0]
+            continue
+        assert torch.isnan(row[[0, 2]]).all() and row[1] == inf
+        large = row[[3, 5]].double()
+        if dtype == torch.float16:
+            assert (large == inf).all()
+        else:
+            want = v[[3, 5]].double()
+            assert ((large - want).abs() <= want * 2 * HALF[dtype]).logical_or(large == inf).all()
+        assert (row[[4, 6, 7, 8]] == 0).all() and 0 <= float(row[9]) <= 1e-44

@@ -141,3 +141,39 @@ def test_channel_far_smaller_than_its_group(cuda, small, n, p, c, groups):
     scale = torch.rand(c, generator=g, device="cuda") + 0.5
     scale[1::4] = small
     _check(x, groups, scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("n,p,c,groups,pitch", [
+    (256, 400, 128, 8, 128),      # a CTA for each image
+    (40, 3000, 128, 4, 136),      # clusters
+    (8, 4096, 320, 32, 320),      # two kernels
+    (30, 900, 70, 7, 75),         # channel by channel
+    (2, 60000, 30, 3, 30),
+    (1, 1, 48, 4, 48)], ids=str)
+def test_float_inputs_with_a_scale(cuda, dtype, n, p, c, groups, pitch):
+    g = torch.Generator(device="cuda").manual_seed(66)
+    wide = (torch.randn(n, p, pitch, generator=g, device="cuda") + 1).to(dtype)
+    x = wide[..., :c]
+    scale = (torch.rand(c + 1, generator=g, device="cuda") * 4 - 2)[1:]   # 4-byte aligned, signed
+    scale[c // 2] = 0
+    _check(x, groups, scale)
+    before = x.clone()
+    ws = torch.empty(m.group_norm_workspace_bytes(x, groups, x), dtype=torch.uint8, device="cuda")
+    want = m.group_norm(x.contiguous(), groups, scale=scale, activation="gelu")
+    m.launch_group_norm(x, groups, x, scale=scale, activation="gelu", workspace=ws,
+                        workspace_bytes=ws.numel())
+    if pitch == c:
+        assert torch.equal(x, want)
+    assert bool(torch.isfinite(x.float()).all()) and not torch.equal(x, before)
+
+
+def test_not_finite_values_under_a_scale_stay_in_their_groups(cuda):
+    x = torch.randn(3, 500, 32, generator=torch.Generator(device="cuda").manual_seed(67), device="cuda")
+    scale = torch.rand(32, device="cuda") + 0.5
+    x[0, 0, 9], x[1, 499, 17], x[2, 250, 25] = float("nan"), float("inf"), -float("inf")
+    y = m.group_norm(x, 4, scale=scale)
+    for image, group in ((0, 1), (1, 2), (2, 3)):
+        bad = torch.isnan(y[image]).view(500, 4, 8).all(2).all(0)
+        assert bad.tolist() == [g == group for g in range(4)]
+        assert int(torch.isnan(y[image]).sum()) == 500 * 8
