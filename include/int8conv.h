@@ -280,8 +280,8 @@ int8conv_status int8conv_launch_quantize_rows(int64_t m, int64_t k, int32_t x_dt
  *   mean_g, var_g over the pixels and the channels of group g = c / (c / groups)
  *   y       = activation((v - mean_g) / sqrt(var_g + eps) * gamma[c] + beta[c])
  * with gamma NULL: 1, beta NULL: 0.  x is BF16, FP16, FP32 or INT32 (what a
- * convolution launch wrote; scale is then what one step of channel c is
- * worth), y BF16, FP16, FP32 or INT8 (with out_scale as for the products).
+ * convolution launch wrote, rounded to fp32 beyond 2^24; scale is then what one
+ * step of channel c is worth), y BF16, FP16, FP32 or INT8 (with out_scale as for the products).
  * Positions are ldx / ldy elements apart (>= channels), images pixels * ldx /
  * pixels * ldy.  channels % groups == 0, channels <= INT8CONV_MAX_NORM_CHANNELS,
  * groups <= INT8CONV_MAX_NORM_GROUPS.
